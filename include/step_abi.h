@@ -1,0 +1,83 @@
+/*
+ * step_abi.h — C ABI of the MI355X (gfx950) operators of a training step that
+ * stand next to the gradient exchange of ring_abi.h: the embedding lookup and
+ * its gradient, the sum of the rows an allgather of sparse gradients delivers,
+ * and the orthogonalised update of a matrix.
+ *
+ * The reference gathers an IndexedSlices instead of reducing it
+ * (tensorflow/contrib/mpi_collectives/__init__.py:146-157) and leaves what
+ * comes before and behind the exchange to the framework around it.
+ *
+ * Conventions, as in ring_abi.h: plain C, an int status, every device entry
+ * point asynchronous on the stream it is given (a hipStream_t as void*; NULL =
+ * the default stream) on the calling thread's current device. Nothing here
+ * allocates, synchronises or keeps anything between calls: scratch memory is
+ * the caller's `workspace`, whose size a *_workspace function tells, so every
+ * call may be recorded into a HIP graph, and calls on several streams are
+ * independent as long as each has a workspace of its own. A workspace needs no
+ * initialisation and starts on a 256-byte boundary.
+ */
+#ifndef STEP_ABI_H_
+#define STEP_ABI_H_
+
+#include <stddef.h>
+#include <stdint.h>
+
+#ifdef __cplusplus
+extern "C" {
+#endif
+
+#define STEP_ABI_VERSION 1
+
+/* Element types; the first three have the codes of enum ring_dtype. */
+enum step_dtype { STEP_F32 = 0, STEP_I32 = 1, STEP_I64 = 2, STEP_BF16 = 3, STEP_F16 = 4 };
+
+/* Status codes, those of enum ring_status. */
+enum step_status {
+  STEP_OK = 0,
+  STEP_ERR_DTYPE = 1,    /* an element type the call does not take */
+  STEP_ERR_ARGUMENT = 2, /* null pointer with a non-zero size, a workspace that is too small ... */
+  STEP_ERR_HIP = 3,      /* a HIP runtime call failed: step_last_hip_error() */
+  STEP_ERR_LIMIT = 5     /* more than 2^31 - 1 tokens or rows, 67,107,840 columns */
+};
+
+int step_abi_version(void);
+const char* step_status_string(int status);
+/* hipError_t of the most recent failing HIP call on this thread (0 if none). */
+int step_last_hip_error(void);
+
+/* ---- embedding ------------------------------------------------------------
+ * Ids are STEP_I32 or STEP_I64, `tokens` of them one behind the other. An id
+ * outside [0, rows) (a padding id of -1, say) reads nothing: its row of the
+ * lookup is zero, and it contributes nothing to a gradient or a sum. Values are
+ * STEP_F32, STEP_BF16 or STEP_F16; the columns of a row are contiguous, rows
+ * are `*_stride` elements apart. */
+
+/* out[t, :] = round(scale * f32(weight[ids[t], :])); out is contiguous. */
+int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const void* weight, int dtype, size_t rows,
+                          size_t width, size_t weight_stride, float scale, void* out, void* stream);
+
+/* out[v, :] = round(scale * sum of f32(grad[t, :]) over the t with ids[t] = v),
+ * for every row v < rows (0 where no token has it). The sum is taken in 32 bits
+ * in the order of t, runs of more than step_embedding_window(tokens) tokens in
+ * pieces of at most that many whose sums are added in order: the same bits on
+ * every call. out is contiguous, of grad's type. */
+size_t step_embedding_window(size_t tokens);
+size_t step_embedding_gradient_workspace(size_t tokens, size_t rows, size_t width);
+int step_embedding_gradient(const void* ids, int id_type, size_t tokens, const void* grad, int dtype, size_t rows,
+                            size_t width, size_t grad_stride, float scale, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream);
+
+/* The same sum with one row for each distinct id in [0, rows), in ascending
+ * order: out_ids[u] (of id_type) and out_values[u, :] for u < *out_count, a
+ * 64-bit count in device memory. out_ids and out_values have room for
+ * min(tokens, rows) rows; what lies behind the last row is left as it was. */
+size_t step_sum_slices_workspace(size_t tokens, size_t rows, size_t width);
+int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* values, int dtype, size_t rows,
+                    size_t width, size_t values_stride, float scale, void* out_ids, void* out_values,
+                    int64_t* out_count, void* workspace, size_t workspace_bytes, void* stream);
+
+#ifdef __cplusplus
+}
+#endif
+#endif /* STEP_ABI_H_ */

@@ -5,6 +5,9 @@
   lib/libring_hip.so      HIP kernels + the C ABI of include/ring_abi.h
                           (csrc/ring_kernels.hip), linked against the HIP
                           runtime only.
+  lib/libstep_hip.so      HIP kernels + the C ABI of include/step_abi.h: the
+                          operators of a training step next to the exchange
+                          (csrc/step_*.hip).
   lib/libmpi_collectives.so
                           the plugin library (csrc/host/*.cc): op registry, the
                           six MPI ops and their kernels, readiness table,
@@ -32,6 +35,8 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 ROOT = os.path.dirname(HERE)
 LIB_DIR = os.path.join(HERE, "lib")
 RING_HIP_SO = os.path.join(LIB_DIR, "libring_hip.so")
+STEP_HIP_SO = os.path.join(LIB_DIR, "libstep_hip.so")
+STEP_SOURCES = ["step_embedding.hip"]
 PLUGIN_SO = os.path.join(LIB_DIR, "libmpi_collectives.so")
 HOST_SOURCES = ["framework.cc", "wire.cc", "ring_driver.cc", "transport.cc", "collective_ops.cc"]
 CXX_FLAGS = ["-O2", "-std=c++17", "-fPIC", "-shared", "-pthread", "-Wall", "-Wextra"]
@@ -51,13 +56,12 @@ def hipcc():
     return exe
 
 
-def build_ring_hip(verbose=True):
+def _build_hip(library, sources, verbose):
     os.makedirs(LIB_DIR, exist_ok=True)
     cmd = [hipcc()] + HIP_FLAGS + [
         "-I", os.path.join(ROOT, "include"),
-        "-o", RING_HIP_SO,
-        os.path.join(HERE, "csrc", "ring_kernels.hip"),
-    ]
+        "-o", library,
+    ] + [os.path.join(HERE, "csrc", f) for f in sources]
     if verbose:
         print(" ".join(cmd), flush=True)
     res = subprocess.run(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
@@ -67,7 +71,15 @@ def build_ring_hip(verbose=True):
         raise RuntimeError("hipcc failed:\n" + out)
     if verbose and out.strip():
         print(out)
-    return RING_HIP_SO
+    return library
+
+
+def build_ring_hip(verbose=True):
+    return _build_hip(RING_HIP_SO, ["ring_kernels.hip"], verbose)
+
+
+def build_step_hip(verbose=True):
+    return _build_hip(STEP_HIP_SO, STEP_SOURCES, verbose)
 
 
 def build_plugin(verbose=True):
@@ -149,7 +161,7 @@ def build_launch_bound_steps(verbose=True):
 
 
 def build_all(verbose=True):
-    return [build_ring_hip(verbose), build_plugin(verbose), build_cpp_gpu_test(verbose),
+    return [build_ring_hip(verbose), build_step_hip(verbose), build_plugin(verbose), build_cpp_gpu_test(verbose),
             build_launch_bound_steps(verbose)]
 
 

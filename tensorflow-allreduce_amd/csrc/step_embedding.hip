@@ -1,0 +1,805 @@
+// Embedding lookup, its gradient by sorted tokens, and the sum of gathered
+// sparse rows for MI355X (gfx950): include/step_abi.h.
+//
+// Mathematics. With ids i_t (t < T) and a table W of V rows of D columns:
+//   lookup     O[t, :]  = round(s * W[i_t, :])
+//   gradient   dW[v, :] = round(s * sum over {t : i_t = v}, in order of t, of G[t, :])
+// One multiplication (addition) per element read: bound by HBM bandwidth, the
+// small calls by their launches.
+//
+// The gradient is gathered, not scattered: atomic additions into dW would
+// serialise on the common tokens, need a float32 image of the whole table and
+// change the result from call to call. Instead the positions are sorted by id
+// (a stable least-significant-digit radix sort of (id, t) pairs, ids first cut
+// to the bits that `rows` needs), which makes the rows of one id a run of
+// ascending t, and every row of dW is summed by the lanes that store it:
+// one read of G, one write of dW, in the table's own type.
+//   * up to kOneGroup tokens one workgroup sorts them in LDS: one launch;
+//   * more tokens take two launches per digit (count, then scatter; the scatter
+//     adds up the counts of all tiles itself instead of a scan in between);
+//   * a run longer than a window (a common token: thousands of rows) is cut at
+//     multiples of the window's length; each window's part is summed by
+//     workgroups of its own into 32 bits and the row's lanes add the parts;
+//   * dW's empty rows are found without clearing a table first: begin[v] is
+//     trusted only if the sorted ids say that a run of v begins there.
+#include "step_common.h"
+
+namespace step {
+namespace {
+
+thread_local int g_last_hip_error = 0;
+
+// A key is an id cut to 32 bits; every id outside [0, rows) becomes `rows`, sorts
+// behind all rows and is dropped there.
+__device__ __forceinline__ uint32_t key_of(const void* ids, int id_type, uint32_t t, uint32_t rows) {
+  if (id_type == STEP_I32) {
+    const uint32_t k = static_cast<const uint32_t*>(ids)[t];  // negative: large
+    return k < rows ? k : rows;
+  }
+  const uint64_t k = static_cast<const uint64_t*>(ids)[t];
+  return k < rows ? static_cast<uint32_t>(k) : rows;
+}
+
+// ---- lookup ---------------------------------------------------------------------
+
+// Lanes of one row of a launch: `lanes` of them, each 16 bytes wide, side by side;
+// a row wider than a workgroup is cut into `chunks` column ranges (grid y).
+struct RowShape {
+  uint32_t lanes, rows_per_group, chunks;
+};
+
+RowShape row_shape(size_t vectors) {
+  RowShape s;
+  s.chunks = static_cast<uint32_t>((vectors + 255) / 256);
+  const size_t per_chunk = (vectors + s.chunks - 1) / s.chunks;
+  if (per_chunk <= 32) {
+    s.lanes = 1;
+    while (s.lanes < per_chunk) s.lanes *= 2;
+  } else {
+    s.lanes = static_cast<uint32_t>(round_up(per_chunk, 64));
+  }
+  s.rows_per_group = 256 / s.lanes;
+  return s;
+}
+
+template <typename T> struct RawOf { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+
+template <typename T> struct Access {
+  // rows of odd widths break 16-byte alignment: element-aligned 16-byte accesses
+  typedef typename RawOf<T>::type Raw;
+  typedef Raw RawU __attribute__((aligned(sizeof(T))));
+  static constexpr int kCount = Vec<T>::kCount;
+
+  static __device__ __forceinline__ Vec<T> load(const T* p, uint32_t count) {
+    Vec<T> v;
+    if (count >= kCount) {
+      v = __builtin_bit_cast(Vec<T>, static_cast<Raw>(*reinterpret_cast<const RawU*>(p)));
+    } else {
+      v = __builtin_bit_cast(Vec<T>, Raw{0, 0, 0, 0});
+      for (int k = 0; k < kCount; k++)
+        if (static_cast<uint32_t>(k) < count) v.at[k] = p[k];
+    }
+    return v;
+  }
+  static __device__ __forceinline__ void store(T* p, Vec<T> v, uint32_t count) {
+    if (count >= kCount) {
+      *reinterpret_cast<RawU*>(p) = __builtin_bit_cast(Raw, v);
+    } else {
+      for (int k = 0; k < kCount; k++)
+        if (static_cast<uint32_t>(k) < count) p[k] = v.at[k];
+    }
+  }
+};
+
+constexpr int kLookupRows = 4;  // rows a lane loads before it stores the first
+
+template <typename T>
+__global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, const T* weight, uint32_t rows,
+                              uint32_t width, uint64_t weight_stride, float scale, T* out, uint32_t lanes,
+                              uint32_t rows_per_group) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t slot = threadIdx.x / lanes;
+  const uint32_t column = (blockIdx.y * lanes + threadIdx.x % lanes) * N;
+  if (slot >= rows_per_group || column >= width) return;
+  const uint32_t count = width - column;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * rows_per_group * kLookupRows + slot;
+  uint32_t key[kLookupRows];
+  Vec<T> v[kLookupRows];
+  for (int k = 0; k < kLookupRows; k++) {
+    const uint64_t t = first + k * rows_per_group;
+    key[k] = t < tokens ? key_of(ids, id_type, static_cast<uint32_t>(t), rows) : rows;
+  }
+  for (int k = 0; k < kLookupRows; k++)
+    v[k] = Access<T>::load(weight + (key[k] < rows ? key[k] : 0) * weight_stride + column, key[k] < rows ? count : 0);
+  for (int k = 0; k < kLookupRows; k++) {
+    const uint64_t t = first + k * rows_per_group;
+    if (t >= tokens) return;
+    for (int e = 0; e < N; e++)
+      v[k].at[e] = from_float<T>(key[k] < rows ? scale * to_float(v[k].at[e]) : 0.f);
+    Access<T>::store(out + t * width + column, v[k], count);
+  }
+}
+
+// ---- sort -------------------------------------------------------------------------
+
+// (a build for the CPU, where every lane is a thread, takes smaller ones)
+#ifndef STEP_SORT_THREADS
+#define STEP_SORT_THREADS 1024
+#define STEP_DIGIT_BITS 9
+#endif
+constexpr int kMostDigitBits = STEP_DIGIT_BITS;
+constexpr int kBins = 1 << kMostDigitBits;
+constexpr uint32_t kSortThreads = STEP_SORT_THREADS;
+constexpr uint32_t kWaves = kSortThreads / 64;
+static_assert(kSortThreads >= static_cast<uint32_t>(kBins), "one lane per digit");
+constexpr uint32_t kOneGroup = 8 * kSortThreads;          // tokens one workgroup sorts in LDS
+constexpr int kTileKeys = 4;                              // keys per lane of a tile of the several-workgroup sort
+constexpr uint32_t kTile = kSortThreads * kTileKeys;
+// above that many tiles each pass would spend its time reading counts; tiles get longer instead
+constexpr uint32_t kMostTiles = 256;
+
+struct Digits {
+  int bits, passes;
+};
+
+// Digits of at most 9 bits: a table of up to 2^18 rows takes two passes.
+Digits digits_for(size_t rows) {
+  int bits = 1;
+  while (bits < 32 && (rows >> bits) != 0) bits++;
+  Digits d;
+  d.passes = (bits + kMostDigitBits - 1) / kMostDigitBits;
+  d.bits = (bits + d.passes - 1) / d.passes;
+  return d;
+}
+
+struct RankScratch {
+  uint16_t count[kWaves][kBins];  // per wave: keys of each digit seen so far, then those in earlier waves (< 2^14)
+  uint32_t total[kBins];
+  uint32_t wave_sum[kWaves];
+};
+
+// The ranks of a round: the number of lanes of this wave before mine with my digit, and their mask. Every lane of the
+// workgroup takes part in every round.
+__device__ __forceinline__ uint64_t same_digit(uint32_t digit, int bits) {
+  uint64_t peers = ~0ull;
+  for (int b = 0; b < bits; b++) {
+    const uint64_t set = __ballot((digit >> b) & 1);
+    peers &= (digit >> b) & 1 ? set : ~set;
+  }
+  return peers;
+}
+
+__device__ __forceinline__ void wave_fence() {
+#if defined(__HIP_DEVICE_COMPILE__)
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+#else
+  __syncthreads();
+#endif
+}
+
+// Counts the digits of `K` keys per lane, wave by wave in order, and leaves in rank[k] the key's place among those of
+// its digit in its wave, in s.count[w][d] how many of digit d stand in waves before w, in s.total[d] the workgroup's
+// count of digit d. A key at or behind `limit` (in the order of the waves' keys) takes no part.
+template <int K>
+__device__ __forceinline__ void rank_keys(RankScratch& s, const uint32_t (&key)[K], uint32_t (&rank)[K], uint32_t first,
+                                          uint32_t limit, int shift, int bits) {
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t bins = 1u << bits;
+  for (uint32_t d = threadIdx.x; d < kWaves * kBins; d += kSortThreads) s.count[d / kBins][d % kBins] = 0;
+  __syncthreads();
+  for (int k = 0; k < K; k++) {
+    const uint32_t digit = (key[k] >> shift) & (bins - 1);
+    const bool here = first + k * 64 + lane < limit;
+    const uint64_t peers = same_digit(digit, bits) & __ballot(here);
+    const uint64_t before = peers & ((1ull << lane) - 1);
+    const uint32_t seen = s.count[wave][digit];
+    wave_fence();
+    rank[k] = seen + static_cast<uint32_t>(__popcll(before));
+    if (here && before == 0) s.count[wave][digit] = static_cast<uint16_t>(seen + __popcll(peers));
+    wave_fence();
+  }
+  __syncthreads();
+  for (uint32_t d = threadIdx.x; d < bins; d += kSortThreads) {
+    uint32_t sum = 0;
+    for (uint32_t w = 0; w < kWaves; w++) {
+      const uint32_t c = s.count[w][d];
+      s.count[w][d] = static_cast<uint16_t>(sum);
+      sum += c;
+    }
+    s.total[d] = sum;
+  }
+  __syncthreads();
+}
+
+// Exclusive prefix sum of x over the workgroup; s.wave_sum is scratch. Every lane takes part.
+__device__ __forceinline__ uint32_t group_scan(RankScratch& s, uint32_t x, uint32_t* sum) {
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  uint32_t up_to = x;
+  for (int step = 1; step < 64; step *= 2) {
+    const uint32_t other = __shfl_up(up_to, step);
+    if (lane >= static_cast<uint32_t>(step)) up_to += other;
+  }
+  if (lane == 63) s.wave_sum[wave] = up_to;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+  for (uint32_t w = 0; w < kWaves; w++) {
+    if (w < wave) before += s.wave_sum[w];
+    all += s.wave_sum[w];
+  }
+  __syncthreads();
+  *sum = all;
+  return before + up_to - x;
+}
+
+// What the sort leaves in the workspace. `order[i]` is the token at place i of the sorted order and `row_of[i]` its row
+// of the output: the id itself (gradient), or the number of its run (sum_slices); ids outside the table stand last,
+// with row_of = rows. Run r covers the places begin[r] .. end[r] - 1 (sum_slices: end[r] is begin[r + 1]).
+struct Sorted {
+  uint32_t* order;
+  uint32_t* row_of;
+  uint32_t* begin;
+  uint32_t* end;
+};
+
+// Everything of the sort in one workgroup's LDS, and the runs.
+template <int K>
+__global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const void* ids, int id_type, uint32_t tokens,
+                                                                uint32_t rows, int bits, int passes, Sorted to,
+                                                                int number_runs, void* out_ids, int64_t* out_count) {
+  __shared__ RankScratch s;
+  __shared__ uint32_t keys[K * kSortThreads];
+  __shared__ uint16_t from[K * kSortThreads];
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t first = wave * 64 * K;
+  uint32_t key[K], token[K], rank[K];
+  for (int k = 0; k < K; k++) {
+    const uint32_t t = first + k * 64 + lane;
+    token[k] = t;
+    key[k] = t < tokens ? key_of(ids, id_type, t, rows) : rows;
+  }
+  for (int pass = 0; pass < passes; pass++) {
+    const int shift = pass * bits;
+    rank_keys<K>(s, key, rank, first, tokens, shift, bits);
+    uint32_t all;
+    const uint32_t d = threadIdx.x;
+    const uint32_t before = group_scan(s, d < (1u << bits) ? s.total[d] : 0, &all);
+    if (d < (1u << bits)) s.total[d] = before;
+    __syncthreads();
+    for (int k = 0; k < K; k++) {
+      if (first + k * 64 + lane >= tokens) continue;
+      const uint32_t digit = (key[k] >> shift) & ((1u << bits) - 1);
+      const uint32_t at = s.total[digit] + s.count[wave][digit] + rank[k];
+      keys[at] = key[k];
+      from[at] = static_cast<uint16_t>(token[k]);
+    }
+    __syncthreads();
+    for (int k = 0; k < K; k++) {
+      const uint32_t t = first + k * 64 + lane;
+      if (t >= tokens) continue;
+      key[k] = keys[t];
+      token[k] = from[t];
+    }
+    // the next pass writes keys[] behind barriers of its own
+  }
+  for (int k = 0; k < K; k++) {
+    const uint32_t i = first + k * 64 + lane;
+    // a run begins at i (and ends at i + 1) if the neighbouring key differs
+    const bool begins = i < tokens && key[k] < rows && (i == 0 || keys[i - 1] != key[k]);
+    const bool ends = i < tokens && key[k] < rows && (i + 1 == tokens || keys[i + 1] != key[k]);
+    rank[k] = (begins ? 1u : 0u) | (ends ? 2u : 0u);
+  }
+  if (!number_runs) {
+    for (int k = 0; k < K; k++) {
+      const uint32_t i = first + k * 64 + lane;
+      if (i >= tokens) continue;
+      to.order[i] = token[k];
+      to.row_of[i] = key[k];
+      if (rank[k] & 1) to.begin[key[k]] = i;
+      if (rank[k] & 2) to.end[key[k]] = i + 1;
+    }
+    return;
+  }
+  // the number of a run: how many begin before it, counted over waves, then rounds, then lanes
+  uint32_t all;
+  uint32_t in_wave = 0;
+  for (int k = 0; k < K; k++) in_wave += static_cast<uint32_t>(__popcll(__ballot(rank[k] & 1)));
+  uint32_t number = group_scan(s, lane == 0 ? in_wave : 0, &all);
+  number = __shfl(number, 0);
+  for (int k = 0; k < K; k++) {
+    const uint32_t i = first + k * 64 + lane;
+    const uint64_t starts = __ballot(rank[k] & 1);
+    const uint32_t up_to = number + static_cast<uint32_t>(__popcll(starts & ((2ull << lane) - 1)));
+    number += static_cast<uint32_t>(__popcll(starts));
+    if (i >= tokens) continue;
+    to.order[i] = token[k];
+    const bool in_table = key[k] < rows;
+    to.row_of[i] = in_table ? up_to - 1 : rows;
+    if (rank[k] & 1) {
+      to.begin[up_to - 1] = i;
+      if (id_type == STEP_I32) static_cast<int32_t*>(out_ids)[up_to - 1] = static_cast<int32_t>(key[k]);
+      else static_cast<int64_t*>(out_ids)[up_to - 1] = key[k];
+    }
+    if ((rank[k] & 2) && (i + 1 == tokens || keys[i + 1] >= rows)) to.begin[all] = i + 1;  // the last run's end
+  }
+  if (threadIdx.x == 0) *out_count = all;
+}
+
+// Several workgroups: the counts of a tile's digits, counts[digit * tiles + tile].
+__global__ void __launch_bounds__(kSortThreads) count_kernel(const void* ids, int id_type, const uint32_t* in_keys,
+                                                             uint32_t tokens, uint32_t rows, uint32_t tile_length,
+                                                             int shift, int bits, uint32_t* counts) {
+  __shared__ uint32_t count[kBins];
+  const uint32_t bins = 1u << bits;
+  if (threadIdx.x < bins) count[threadIdx.x] = 0;
+  __syncthreads();
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tile_length;
+  for (uint32_t j = threadIdx.x; j < tile_length; j += kSortThreads) {
+    const uint64_t t = first + j;
+    if (t >= tokens) break;
+    const uint32_t key = in_keys ? in_keys[t] : key_of(ids, id_type, static_cast<uint32_t>(t), rows);
+    atomicAdd(&count[(key >> shift) & (bins - 1)], 1u);
+  }
+  __syncthreads();
+  if (threadIdx.x < bins) counts[static_cast<uint64_t>(threadIdx.x) * gridDim.x + blockIdx.x] = count[threadIdx.x];
+}
+
+// The scatter of a digit's pass. A digit's keys of this tile go behind all smaller digits' keys and those of the same
+// digit in earlier tiles.
+__global__ void __launch_bounds__(kSortThreads) scatter_kernel(const void* ids, int id_type, const uint32_t* in_keys,
+                                                               const uint32_t* in_order, uint32_t tokens, uint32_t rows,
+                                                               uint32_t tile_length, int shift, int bits,
+                                                               const uint32_t* counts, uint32_t* out_keys,
+                                                               uint32_t* out_order) {
+  __shared__ RankScratch s;
+  __shared__ uint32_t base[kBins];
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t bins = 1u << bits;
+  uint32_t in_earlier = 0, in_all = 0;
+  if (threadIdx.x < bins) {
+    const uint32_t* row = counts + static_cast<uint64_t>(threadIdx.x) * gridDim.x;
+    for (uint32_t b = 0; b < gridDim.x; b++) {
+      const uint32_t c = row[b];
+      if (b < blockIdx.x) in_earlier += c;
+      in_all += c;
+    }
+  }
+  uint32_t all;
+  const uint32_t smaller = group_scan(s, in_all, &all);
+  if (threadIdx.x < bins) base[threadIdx.x] = smaller + in_earlier;
+  __syncthreads();
+  const uint64_t tile = static_cast<uint64_t>(blockIdx.x) * tile_length;
+  for (uint32_t part = 0; part < tile_length; part += kTile) {
+    const uint64_t at0 = tile + part;
+    const uint32_t here = at0 >= tokens ? 0 : tokens - at0 < kTile ? static_cast<uint32_t>(tokens - at0) : kTile;
+    const uint32_t first = wave * 64 * kTileKeys;
+    uint32_t key[kTileKeys], token[kTileKeys], rank[kTileKeys];
+    for (int k = 0; k < kTileKeys; k++) {
+      const uint32_t j = first + k * 64 + lane;
+      key[k] = rows;
+      token[k] = 0;
+      if (j < here) {
+        const uint32_t t = static_cast<uint32_t>(at0 + j);
+        key[k] = in_keys ? in_keys[t] : key_of(ids, id_type, t, rows);
+        token[k] = in_order ? in_order[t] : t;
+      }
+    }
+    rank_keys<kTileKeys>(s, key, rank, first, here, shift, bits);
+    for (int k = 0; k < kTileKeys; k++) {
+      if (first + k * 64 + lane >= here) continue;
+      const uint32_t digit = (key[k] >> shift) & (bins - 1);
+      const uint32_t at = base[digit] + s.count[wave][digit] + rank[k];
+      out_keys[at] = key[k];
+      out_order[at] = token[k];
+    }
+    __syncthreads();
+    if (threadIdx.x < bins) base[threadIdx.x] += s.total[threadIdx.x];
+    __syncthreads();
+  }
+}
+
+// The runs of the sorted keys. counts == nullptr: begin/end by key. Otherwise a run's number is its rank: a first
+// launch (number == 0) counts the runs that begin in each tile, a second numbers them.
+__global__ void __launch_bounds__(kSortThreads) runs_kernel(const uint32_t* keys, uint32_t tokens, uint32_t rows,
+                                                            Sorted to) {
+  const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kSortThreads + threadIdx.x;
+  if (i >= tokens) return;
+  const uint32_t key = keys[i];
+  if (key >= rows) return;
+  if (i == 0 || keys[i - 1] != key) to.begin[key] = static_cast<uint32_t>(i);
+  if (i + 1 == tokens || keys[i + 1] != key) to.end[key] = static_cast<uint32_t>(i + 1);
+}
+
+__device__ __forceinline__ bool begins_run(const uint32_t* keys, uint64_t i, uint32_t tokens, uint32_t rows) {
+  if (i >= tokens) return false;
+  const uint32_t key = keys[i];
+  return key < rows && (i == 0 || keys[i - 1] != key);
+}
+
+__global__ void __launch_bounds__(kSortThreads) count_runs_kernel(const uint32_t* keys, uint32_t tokens, uint32_t rows,
+                                                                  uint32_t tile_length, uint32_t* counts) {
+  __shared__ RankScratch s;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * tile_length;
+  uint32_t mine = 0;
+  for (uint32_t j = threadIdx.x; j < tile_length; j += kSortThreads) mine += begins_run(keys, first + j, tokens, rows);
+  uint32_t all;
+  group_scan(s, mine, &all);
+  if (threadIdx.x == 0) counts[blockIdx.x] = all;
+}
+
+__global__ void __launch_bounds__(kSortThreads) number_runs_kernel(const uint32_t* keys, uint32_t tokens, uint32_t rows,
+                                                                   uint32_t tile_length, const uint32_t* counts, Sorted to,
+                                                                   int id_type, void* out_ids, int64_t* out_count) {
+  __shared__ RankScratch s;
+  uint32_t earlier = 0, in_all = 0;
+  for (uint32_t b = threadIdx.x; b < gridDim.x; b += kSortThreads) {
+    const uint32_t c = counts[b];
+    in_all += c;
+    if (b < blockIdx.x) earlier += c;
+  }
+  uint32_t number, total;
+  group_scan(s, earlier, &number);
+  group_scan(s, in_all, &total);
+  const uint64_t tile = static_cast<uint64_t>(blockIdx.x) * tile_length;
+  for (uint32_t part = 0; part < tile_length; part += kSortThreads) {
+    const uint64_t i = tile + part + threadIdx.x;
+    const bool begins = begins_run(keys, i, tokens, rows);
+    uint32_t here;
+    const uint32_t before = group_scan(s, begins ? 1 : 0, &here);
+    if (i < tokens) {
+      const uint32_t key = keys[i];
+      const uint32_t run = number + before + (begins ? 1 : 0) - 1;
+      to.row_of[i] = key < rows ? run : rows;
+      if (begins) {
+        to.begin[run] = static_cast<uint32_t>(i);
+        if (id_type == STEP_I32) static_cast<int32_t*>(out_ids)[run] = static_cast<int32_t>(key);
+        else static_cast<int64_t*>(out_ids)[run] = key;
+      }
+      if (key < rows && (i + 1 == tokens || keys[i + 1] >= rows)) to.begin[total] = static_cast<uint32_t>(i + 1);
+    }
+    number += here;
+  }
+  if (blockIdx.x == 0 && threadIdx.x == 0) *out_count = total;
+}
+
+// ---- sums ------------------------------------------------------------------------
+
+// acc += the rows order[b] .. order[e - 1] of `values`, in that order, at one lane's columns.
+template <typename T>
+__device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::kCount], const T* values, uint64_t stride,
+                                         const uint32_t* order, uint32_t b, uint32_t e, uint32_t count) {
+  constexpr int N = Vec<T>::kCount;
+  auto add = [&](auto steps) {
+    constexpr int U = decltype(steps)::value;
+    Vec<T> v[U];
+    for (int k = 0; k < U; k++) v[k] = Access<T>::load(values + order[b + k] * stride, count);
+    for (int k = 0; k < U; k++)
+      for (int n = 0; n < N; n++) acc[n] += to_float(v[k].at[n]);
+    b += U;
+  };
+  while (e - b >= 8) add(std::integral_constant<int, 8>());
+  if (e - b >= 4) add(std::integral_constant<int, 4>());
+  if (e - b >= 2) add(std::integral_constant<int, 2>());
+  if (e - b >= 1) add(std::integral_constant<int, 1>());
+}
+
+// The parts of long runs: window j holds the places j * window .. of the sorted order. At most two long runs have a
+// part in it, that of its first place (parts[2 j]) and that of its last (parts[2 j + 1]).
+template <typename T>
+__global__ void window_kernel(const T* values, uint64_t stride, uint32_t tokens, uint32_t rows, uint32_t width, Sorted by,
+                              int numbered, uint32_t window, uint32_t lanes, float* parts, uint64_t parts_stride) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t column = (blockIdx.y * lanes + threadIdx.x) * N;
+  if (column >= width) return;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * window;
+  const uint32_t last = tokens - first < window ? tokens - 1 : static_cast<uint32_t>(first) + window - 1;
+  for (int side = 0; side < 2; side++) {
+    const uint32_t place = side ? last : static_cast<uint32_t>(first);
+    const uint32_t run = by.row_of[place];
+    if (run >= rows || (side && run == by.row_of[first])) continue;
+    const uint32_t b = by.begin[run], e = numbered ? by.begin[run + 1] : by.end[run];
+    if (e - b <= window) continue;
+    float acc[N] = {};
+    add_rows<T>(acc, values + column, stride, by.order, b > first ? b : static_cast<uint32_t>(first),
+                e <= last ? e : last + 1, width - column);
+    float* to = parts + (static_cast<uint64_t>(blockIdx.x) * 2 + side) * parts_stride + column;
+    for (int n = 0; n < N; n++) to[n] = acc[n];
+  }
+}
+
+constexpr int kSumRows = 4;  // rows of a lane slot
+
+template <typename T, bool NUMBERED>
+__global__ void sum_kernel(const T* values, uint64_t stride, uint32_t tokens, uint32_t rows, uint32_t width, float scale,
+                           Sorted by, const int64_t* run_count, uint32_t window, const float* parts,
+                           uint64_t parts_stride, T* out, uint32_t lanes, uint32_t rows_per_group) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t slot = threadIdx.x / lanes;
+  const uint32_t column = (blockIdx.y * lanes + threadIdx.x % lanes) * N;
+  if (slot >= rows_per_group || column >= width) return;
+  const uint32_t count = width - column;
+  const uint64_t runs = NUMBERED ? static_cast<uint64_t>(*run_count) : rows;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * rows_per_group * kSumRows + slot;
+  uint32_t b[kSumRows], e[kSumRows];
+  for (int k = 0; k < kSumRows; k++) {
+    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
+    b[k] = r < runs ? by.begin[r] : 0xffffffffu;
+  }
+  for (int k = 0; k < kSumRows; k++) {
+    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
+    e[k] = 0;
+    if (r >= runs) continue;
+    if (NUMBERED) {
+      e[k] = by.begin[r + 1];
+    } else {
+      // begin[r] holds anything if no token has row r: a run of r begins there only if the sorted ids say so
+      const bool begins = b[k] < tokens && by.row_of[b[k]] == r && (b[k] == 0 || by.row_of[b[k] - 1] != r);
+      if (begins) e[k] = by.end[r];
+      else b[k] = 0;
+    }
+  }
+  for (int k = 0; k < kSumRows; k++) {
+    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
+    if (r >= runs) return;
+    float acc[N] = {};
+    if (e[k] - b[k] <= window) {
+      add_rows<T>(acc, values + column, stride, by.order, b[k], e[k], count);
+    } else {
+      for (uint32_t j = b[k] / window; j <= (e[k] - 1) / window; j++) {
+        const uint64_t part = static_cast<uint64_t>(j) * 2 + (b[k] > j * window ? 1 : 0);
+        for (int n = 0; n < N; n++) acc[n] += parts[part * parts_stride + column + n];
+      }
+    }
+    Vec<T> v;
+    for (int n = 0; n < N; n++) v.at[n] = from_float<T>(scale * acc[n]);
+    Access<T>::store(out + r * width + column, v, count);
+  }
+}
+
+// ---- host side --------------------------------------------------------------------
+
+// The pieces of a workspace, each on a 256-byte boundary.
+struct Layout {
+  size_t keys[2], order[2], counts, row_of, begin, end, parts, bytes;
+  uint32_t tile_length, tiles, window, windows;
+  size_t parts_stride;
+};
+
+uint32_t window_for(size_t tokens) {
+  // a long run costs tokens / windows row additions in a row, then one for each window: balanced at the square root
+  uint32_t w = 64;
+  while (static_cast<size_t>(w) * w < tokens) w *= 2;
+  return w;
+}
+
+Layout layout_for(size_t tokens, size_t rows, size_t width, bool numbered) {
+  Layout l = {};
+  size_t at = 0;
+  auto take = [&at](size_t bytes) {
+    const size_t here = at;
+    at += round_up(bytes, 256);
+    return here;
+  };
+  l.window = window_for(tokens);
+  l.windows = static_cast<uint32_t>((tokens + l.window - 1) / l.window);
+  l.tile_length = kTile;
+  if (tokens > static_cast<size_t>(kTile) * kMostTiles)
+    l.tile_length = static_cast<uint32_t>(round_up((tokens + kMostTiles - 1) / kMostTiles, kTile));
+  l.tiles = static_cast<uint32_t>((tokens + l.tile_length - 1) / l.tile_length);
+  const bool one = tokens <= kOneGroup;
+  for (int k = 0; k < 2; k++) {
+    l.keys[k] = take(one ? (k ? 0 : tokens * 4) : tokens * 4);
+    l.order[k] = take(one ? (k ? 0 : tokens * 4) : tokens * 4);
+  }
+  l.counts = take(one ? 0 : static_cast<size_t>(kBins) * l.tiles * 4);
+  l.row_of = numbered && !one ? take(tokens * 4) : l.keys[0];
+  const size_t runs = numbered ? (tokens < rows ? tokens : rows) + 1 : rows;
+  l.begin = take(runs * 4);
+  l.end = numbered ? l.begin : take(runs * 4);
+  l.parts_stride = round_up(width, 64);
+  l.parts = take(tokens > l.window ? static_cast<size_t>(l.windows) * 2 * l.parts_stride * 4 : 0);
+  l.bytes = at ? at : 256;
+  return l;
+}
+
+// Sorts the tokens and finds their runs. *numbered: see Sorted.
+Sorted sort_tokens(const Layout& l, char* ws, const void* ids, int id_type, uint32_t tokens, uint32_t rows, bool numbered,
+                   void* out_ids, int64_t* out_count, hipStream_t stream) {
+  auto at = [ws](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
+  const Digits d = digits_for(rows);
+  Sorted to = {at(l.order[0]), at(l.row_of), at(l.begin), at(l.end)};
+  if (tokens <= kOneGroup) {
+    auto sort = [&](auto keys) {
+      hipLaunchKernelGGL((sort_one_kernel<decltype(keys)::value>), dim3(1), dim3(kSortThreads), 0, stream, ids, id_type,
+                         tokens, rows, d.bits, d.passes, to, numbered ? 1 : 0, out_ids, out_count);
+    };
+    if (tokens <= kSortThreads) sort(std::integral_constant<int, 1>());
+    else if (tokens <= 2 * kSortThreads) sort(std::integral_constant<int, 2>());
+    else if (tokens <= 4 * kSortThreads) sort(std::integral_constant<int, 4>());
+    else sort(std::integral_constant<int, 8>());
+    return to;
+  }
+  const uint32_t* keys = nullptr;
+  const uint32_t* order = nullptr;
+  // the last pass ends in buffer 0
+  for (int pass = 0; pass < d.passes; pass++) {
+    const int into = (d.passes - 1 - pass) & 1;
+    hipLaunchKernelGGL(count_kernel, dim3(l.tiles), dim3(kSortThreads), 0, stream, ids, id_type, keys, tokens, rows,
+                       l.tile_length, pass * d.bits, d.bits, at(l.counts));
+    hipLaunchKernelGGL(scatter_kernel, dim3(l.tiles), dim3(kSortThreads), 0, stream, ids, id_type, keys, order, tokens,
+                       rows, l.tile_length, pass * d.bits, d.bits, static_cast<const uint32_t*>(at(l.counts)),
+                       at(l.keys[into]), at(l.order[into]));
+    keys = at(l.keys[into]);
+    order = at(l.order[into]);
+  }
+  if (!numbered) {
+    hipLaunchKernelGGL(runs_kernel, dim3((tokens + kSortThreads - 1) / kSortThreads), dim3(kSortThreads), 0, stream, keys,
+                       tokens, rows, to);
+  } else {
+    hipLaunchKernelGGL(count_runs_kernel, dim3(l.tiles), dim3(kSortThreads), 0, stream, keys, tokens, rows, l.tile_length,
+                       at(l.counts));
+    hipLaunchKernelGGL(number_runs_kernel, dim3(l.tiles), dim3(kSortThreads), 0, stream, keys, tokens, rows,
+                       l.tile_length, static_cast<const uint32_t*>(at(l.counts)), to, id_type, out_ids, out_count);
+  }
+  return to;
+}
+
+template <typename T, bool NUMBERED>
+void sum_rows(const Layout& l, char* ws, const Sorted& by, const void* values, uint64_t stride, uint32_t tokens,
+              uint32_t rows, uint32_t width, float scale, const int64_t* run_count, void* out, hipStream_t stream) {
+  const size_t vectors = (width + Vec<T>::kCount - 1) / Vec<T>::kCount;
+  float* parts = reinterpret_cast<float*>(ws + l.parts);
+  if (tokens > l.window) {
+    RowShape w = row_shape(vectors);
+    // one row of lanes per workgroup, whole waves of it
+    const uint32_t threads = w.lanes < 64 ? 64 : w.lanes;
+    hipLaunchKernelGGL((window_kernel<T>), dim3(l.windows, w.chunks), dim3(threads), 0, stream,
+                       static_cast<const T*>(values), stride, tokens, rows, width, by, NUMBERED ? 1 : 0, l.window, threads,
+                       parts, static_cast<uint64_t>(l.parts_stride));
+  }
+  const RowShape s = row_shape(vectors);
+  const uint64_t most = NUMBERED ? (tokens < rows ? tokens : rows) : rows;
+  const uint64_t per_group = static_cast<uint64_t>(s.rows_per_group) * kSumRows;
+  hipLaunchKernelGGL((sum_kernel<T, NUMBERED>), dim3(static_cast<uint32_t>((most + per_group - 1) / per_group), s.chunks),
+                     dim3(256), 0, stream, static_cast<const T*>(values), stride, tokens, rows, width, scale, by, run_count,
+                     l.window, static_cast<const float*>(parts), static_cast<uint64_t>(l.parts_stride),
+                     static_cast<T*>(out), s.lanes, s.rows_per_group);
+}
+
+__global__ void zero_kernel(uint32_t* to, uint64_t words, uint16_t* tail, int has_tail) {
+  const uint64_t step = static_cast<uint64_t>(gridDim.x) * blockDim.x;
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
+  for (uint64_t i = first; i < words; i += step) to[i] = 0;
+  if (has_tail && first == 0) *tail = 0;
+}
+
+// A row's column ranges are grid y: 65535 of 256 lanes.
+constexpr size_t kMostWidth = static_cast<size_t>(65535) * 256 * 4;
+
+int check(const void* ids, int id_type, size_t tokens, const void* values, int dtype, size_t rows, size_t width,
+          size_t stride) {
+  if (id_type != STEP_I32 && id_type != STEP_I64) return STEP_ERR_DTYPE;
+  if (!is_float(dtype)) return STEP_ERR_DTYPE;
+  if (tokens > kMostSize || rows > kMostSize || width > kMostSize) return STEP_ERR_LIMIT;
+  if (tokens && !ids) return STEP_ERR_ARGUMENT;
+  if (width > kMostWidth) return STEP_ERR_LIMIT;
+  if (stride < width) return STEP_ERR_ARGUMENT;
+  if (!values && width && tokens) return STEP_ERR_ARGUMENT;
+  return STEP_OK;
+}
+
+}  // namespace
+
+int hip_fail(hipError_t e) {
+  g_last_hip_error = static_cast<int>(e);
+  return STEP_ERR_HIP;
+}
+
+}  // namespace step
+
+using namespace step;
+
+extern "C" {
+
+int step_abi_version(void) { return STEP_ABI_VERSION; }
+
+const char* step_status_string(int status) {
+  switch (status) {
+    case STEP_OK: return "ok";
+    case STEP_ERR_DTYPE: return "Invalid tensor type passed.";
+    case STEP_ERR_ARGUMENT: return "invalid argument";
+    case STEP_ERR_HIP: return "HIP runtime call failed";
+    case STEP_ERR_LIMIT: return "more than 2^31 - 1 tokens or rows, or 67107840 columns";
+    default: return "unknown status";
+  }
+}
+
+int step_last_hip_error(void) { return g_last_hip_error; }
+
+int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const void* weight, int dtype, size_t rows,
+                          size_t width, size_t weight_stride, float scale, void* out, void* stream) {
+  int rc = check(ids, id_type, tokens, rows ? weight : ids, dtype, rows, width, weight_stride);
+  if (rc != STEP_OK) return rc;
+  if (tokens == 0 || width == 0) return STEP_OK;
+  if (!out) return STEP_ERR_ARGUMENT;
+  const RowShape s = row_shape((width * dtype_size(dtype) + 15) / 16);
+  const size_t per_group = static_cast<size_t>(s.rows_per_group) * kLookupRows;
+  const dim3 grid(static_cast<uint32_t>((tokens + per_group - 1) / per_group), s.chunks);
+  auto go = [&](auto type) {
+    typedef decltype(type) T;
+    hipLaunchKernelGGL((lookup_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), ids, id_type,
+                       static_cast<uint32_t>(tokens), static_cast<const T*>(weight), static_cast<uint32_t>(rows),
+                       static_cast<uint32_t>(width), static_cast<uint64_t>(weight_stride), scale, static_cast<T*>(out),
+                       s.lanes, s.rows_per_group);
+  };
+  if (dtype == STEP_F32) go(F32());
+  else if (dtype == STEP_BF16) go(BF16());
+  else go(F16());
+  return launched();
+}
+
+size_t step_embedding_window(size_t tokens) { return window_for(tokens); }
+
+size_t step_embedding_gradient_workspace(size_t tokens, size_t rows, size_t width) {
+  if (tokens > kMostSize || rows > kMostSize || width > kMostSize) return 0;
+  return layout_for(tokens, rows, width, false).bytes;
+}
+
+int step_embedding_gradient(const void* ids, int id_type, size_t tokens, const void* grad, int dtype, size_t rows,
+                            size_t width, size_t grad_stride, float scale, void* out, void* workspace,
+                            size_t workspace_bytes, void* stream_) {
+  const int rc = check(ids, id_type, tokens, grad, dtype, rows, width, grad_stride);
+  if (rc != STEP_OK) return rc;
+  if (rows == 0 || width == 0) return STEP_OK;
+  if (!out) return STEP_ERR_ARGUMENT;
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (tokens == 0) {
+    const uint64_t bytes = static_cast<uint64_t>(rows) * width * dtype_size(dtype), words = bytes / 4;
+    const uint64_t groups = (words + 255) / 256;
+    hipLaunchKernelGGL(zero_kernel, dim3(static_cast<uint32_t>(groups < 1 ? 1 : groups > 4096 ? 4096 : groups)), dim3(256),
+                       0, stream, static_cast<uint32_t*>(out), words,
+                       reinterpret_cast<uint16_t*>(static_cast<char*>(out) + words * 4), bytes % 4 ? 1 : 0);
+    return launched();
+  }
+  const Layout l = layout_for(tokens, rows, width, false);
+  if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
+  char* ws = static_cast<char*>(workspace);
+  const uint32_t t = static_cast<uint32_t>(tokens), v = static_cast<uint32_t>(rows), w = static_cast<uint32_t>(width);
+  const Sorted by = sort_tokens(l, ws, ids, id_type, t, v, false, nullptr, nullptr, stream);
+  if (dtype == STEP_F32) sum_rows<F32, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
+  else if (dtype == STEP_BF16) sum_rows<BF16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
+  else sum_rows<F16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
+  return launched();
+}
+
+size_t step_sum_slices_workspace(size_t tokens, size_t rows, size_t width) {
+  if (tokens > kMostSize || rows > kMostSize || width > kMostSize) return 0;
+  return layout_for(tokens, rows, width, true).bytes;
+}
+
+int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* values, int dtype, size_t rows, size_t width,
+                    size_t values_stride, float scale, void* out_ids, void* out_values, int64_t* out_count,
+                    void* workspace, size_t workspace_bytes, void* stream_) {
+  const int rc = check(ids, id_type, tokens, values, dtype, rows, width, values_stride);
+  if (rc != STEP_OK) return rc;
+  if (!out_count) return STEP_ERR_ARGUMENT;
+  hipStream_t stream = static_cast<hipStream_t>(stream_);
+  if (tokens == 0 || rows == 0) {
+    hipLaunchKernelGGL(zero_kernel, dim3(1), dim3(256), 0, stream, reinterpret_cast<uint32_t*>(out_count),
+                       static_cast<uint64_t>(2), static_cast<uint16_t*>(nullptr), 0);
+    return launched();
+  }
+  if (!out_ids || (width && !out_values)) return STEP_ERR_ARGUMENT;
+  const Layout l = layout_for(tokens, rows, width, true);
+  if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
+  char* ws = static_cast<char*>(workspace);
+  const uint32_t t = static_cast<uint32_t>(tokens), v = static_cast<uint32_t>(rows), w = static_cast<uint32_t>(width);
+  const Sorted by = sort_tokens(l, ws, ids, id_type, t, v, true, out_ids, out_count, stream);
+  if (width == 0) return launched();
+  if (dtype == STEP_F32) sum_rows<F32, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
+  else if (dtype == STEP_BF16) sum_rows<BF16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
+  else sum_rows<F16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
+  return launched();
+}
+
+}  // extern "C"

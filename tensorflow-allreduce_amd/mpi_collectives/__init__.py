@@ -31,6 +31,9 @@ collectives complete at once.
 @@allreduce
 @@allreduce_batch
 @@allgather
+@@embedding
+@@embedding_gradient
+@@sum_slices
 """
 import contextlib
 import os
@@ -42,6 +45,7 @@ from . import _plugin, mpi_ops, ring_abi
 from ._plugin import (FailedPreconditionError, InternalError, InvalidArgumentError,  # noqa: F401
                       NotFoundError, OpError, UnknownError)
 from .mpi_ops import _allreduce, allgather, init, local_rank, rank, size  # noqa: F401
+from .step_ops import IndexedSlices, embedding, embedding_gradient, sum_slices  # noqa: F401
 
 _TORCH2RING = {torch.float32: ring_abi.F32, torch.int32: ring_abi.I32, torch.int64: ring_abi.I64}
 
@@ -89,14 +93,6 @@ class PendingTensor:
         if self._error is not None:
             raise self._error
         return self._value
-
-
-class IndexedSlices:
-    """A sparse representation of a set of tensor slices at given indices
-    (the tf.IndexedSlices the reference's allreduce accepts)."""
-
-    def __init__(self, values, indices, dense_shape=None):
-        self.values, self.indices, self.dense_shape = values, indices, dense_shape
 
 
 def _env_size():
@@ -671,6 +667,16 @@ def prepare_allreduce_batch(tensors, average=True, inplace=False):
     return AllreduceBatch(tensors, average=average, inplace=inplace)
 
 
+def _coalesced(g):
+    """g.coalesce(), without its sort where the indices ascend already (autograd drops that mark when it stores a
+    gradient, embedding's among them)."""
+    if not g.is_coalesced() and g.sparse_dim() == 1:
+        index = g._indices()[0]
+        if bool((index[1:] > index[:-1]).all()):
+            return torch.sparse_coo_tensor(g._indices(), g._values(), g.shape, is_coalesced=True, check_invariants=False)
+    return g.coalesce()
+
+
 class DistributedOptimizer:
     """An optimizer that wraps a torch.optim.Optimizer, using an MPI allreduce
     to average gradient values before applying gradients to model weights
@@ -725,7 +731,7 @@ class DistributedOptimizer:
         for p in params:
             g = p.grad
             if g.is_sparse:
-                g = g.coalesce()
+                g = _coalesced(g)
                 slices = IndexedSlices(g.values().contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape)
                 out.append((allreduce(slices), p))
             else:
@@ -802,8 +808,10 @@ class DistributedOptimizer:
         for g, p in grads_and_vars:
             g = _resolve(g.resolve() if isinstance(g, _FusedGrad) else g)
             if isinstance(g, IndexedSlices):
-                idx = g.indices.reshape(1, -1)
-                p.grad = torch.sparse_coo_tensor(idx, g.values, size=tuple(g.dense_shape)).coalesce()
+                # every rank's rows, one behind the other: one row for each index, the ranks' rows added in order
+                total = sum_slices(g)
+                p.grad = torch.sparse_coo_tensor(total.indices.long().reshape(1, -1), total.values,
+                                                 size=tuple(g.dense_shape), is_coalesced=True)
             else:
                 p.grad = g.reshape(p.shape)
         return self._optimizer.step()

@@ -1,0 +1,236 @@
+"""Operators of a training step around the gradient exchange, over torch
+tensors on the GPU: the embedding lookup and its gradient, and the sum of the
+rows that allreduce(IndexedSlices) gathers.
+
+They run on torch's current stream of the tensors' device, allocate through
+torch and synchronise nothing (except where a result's size depends on the
+data: sum_slices, and the sparse gradient of embedding).
+"""
+import torch
+
+from . import step_abi
+from ._plugin import InvalidArgumentError
+
+_FLOATS = {torch.float32: step_abi.F32, torch.bfloat16: step_abi.BF16, torch.float16: step_abi.F16}
+_IDS = {torch.int32: step_abi.I32, torch.int64: step_abi.I64}
+
+
+class IndexedSlices:
+    """A sparse representation of a set of tensor slices at given indices
+    (the tf.IndexedSlices the reference's allreduce accepts)."""
+
+    def __init__(self, values, indices, dense_shape=None):
+        self.values, self.indices, self.dense_shape = values, indices, dense_shape
+
+
+def _refuse(why, *args):
+    raise InvalidArgumentError(why % args)
+
+
+def _check_tensor(t, name, types, what):
+    if not isinstance(t, torch.Tensor):
+        _refuse("%s: %s must be a torch.Tensor, got %s", what, name, type(t).__name__)
+    if t.dtype not in types:
+        _refuse("%s: %s has type %s; it takes %s", what, name, t.dtype, ", ".join(str(k) for k in types))
+    if not t.is_cuda:
+        _refuse("%s: %s is on %s; there are GPU kernels only", what, name, t.device)
+
+
+def _same_device(what, a, b):
+    if a.device != b.device:
+        _refuse("%s: tensors on %s and %s", what, a.device, b.device)
+
+
+def _rows_of(t):
+    """`t` as rows whose columns are contiguous and which are t.stride(0) apart, copied only if it is not."""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+class _on:
+    """The tensors' device as the current one (entered only if it is not), and its current stream."""
+
+    def __init__(self, device):
+        self._index = device.index
+        self._guard = None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self._index:
+            self._guard = torch.cuda.device(self._index)
+            self._guard.__enter__()
+        return torch.cuda.current_stream(self._index).cuda_stream
+
+    def __exit__(self, *exc):
+        if self._guard is not None:
+            self._guard.__exit__(*exc)
+        return False
+
+
+def _workspace(size, device):
+    return torch.empty(size, dtype=torch.uint8, device=device)
+
+
+def _lookup(ids, weight, scale):
+    ids = ids.contiguous()
+    weight, stride = _rows_of(weight)
+    rows, width = weight.shape
+    out = torch.empty(ids.shape + (width,), dtype=weight.dtype, device=weight.device)
+    with _on(weight.device) as stream:
+        step_abi.check(step_abi.lib().step_embedding_lookup(
+            ids.data_ptr(), _IDS[ids.dtype], ids.numel(), weight.data_ptr(), _FLOATS[weight.dtype], rows, width, stride,
+            scale, out.data_ptr(), stream), "embedding")
+    return out
+
+
+def embedding_gradient(grad, ids, rows, scale=1.0):
+    """The dense gradient of `embedding` with respect to its table: row v of the
+    result is scale * the sum of the rows of `grad` whose id is v, 0 if there is
+    none.
+
+    Arguments:
+        grad: gradient of the lookup's result, ids.shape + (width,), float32,
+              bfloat16 or float16. Its last dimension should be contiguous (it
+              is copied otherwise).
+        ids: int32 or int64 tensor; ids outside [0, rows) contribute nothing.
+        rows: rows of the table.
+        scale: as in `embedding`.
+
+    Sums are taken in 32 bits in the order of the tokens and rounded once to
+    grad's type; the same call gives the same bits every time."""
+    what = "embedding_gradient"
+    _check_tensor(grad, "grad", _FLOATS, what)
+    _check_tensor(ids, "ids", _IDS, what)
+    _same_device(what, grad, ids)
+    rows = int(rows)
+    if rows < 0:
+        _refuse("%s: rows is %d", what, rows)
+    if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
+        _refuse("%s: a gradient of shape %s for ids of shape %s", what, tuple(grad.shape), tuple(ids.shape))
+    return _gradient(grad, ids, rows, float(scale))
+
+
+def _gradient(grad, ids, rows, scale):
+    ids = ids.contiguous()
+    width = grad.shape[-1]
+    grad, stride = _rows_of(grad.reshape(-1, width) if grad.numel() else grad.new_empty(ids.numel(), width))
+    tokens = grad.shape[0]
+    out = torch.empty(rows, width, dtype=grad.dtype, device=grad.device)
+    L = step_abi.lib()
+    with _on(grad.device) as stream:
+        size = L.step_embedding_gradient_workspace(tokens, rows, width)
+        ws = _workspace(size, grad.device)
+        step_abi.check(L.step_embedding_gradient(
+            ids.data_ptr(), _IDS[ids.dtype], tokens, grad.data_ptr(), _FLOATS[grad.dtype], rows, width, stride, scale,
+            out.data_ptr(), ws.data_ptr(), size, stream), "embedding_gradient")
+    return out
+
+
+def sum_slices(slices):
+    """An IndexedSlices with one row for each distinct index, in ascending order:
+    the sum of the rows of `slices` that have it. This is what makes a gradient
+    of what allreduce(IndexedSlices) delivers, where every rank's rows stand one
+    behind the other.
+
+    Arguments:
+        slices: IndexedSlices with values of shape (n, ...), float32, bfloat16 or
+                float16, indices of shape (n,), int32 or int64, and dense_shape
+                set. Rows whose index is outside [0, dense_shape[0]) are left out.
+
+    Sums are taken in 32 bits in the order of the rows and rounded once; the
+    same call gives the same bits every time. The number of distinct indices is
+    read from the GPU, so the call waits for its stream and cannot be captured
+    into a graph."""
+    what = "sum_slices"
+    if not isinstance(slices, IndexedSlices):
+        _refuse("%s: an IndexedSlices is needed, got %s", what, type(slices).__name__)
+    values, indices = slices.values, slices.indices
+    _check_tensor(values, "values", _FLOATS, what)
+    _check_tensor(indices, "indices", _IDS, what)
+    _same_device(what, values, indices)
+    if slices.dense_shape is None:
+        _refuse("%s: dense_shape is needed", what)
+    shape = tuple(int(d) for d in slices.dense_shape)
+    if indices.dim() != 1 or values.dim() < 1 or values.shape[0] != indices.shape[0] or tuple(values.shape[1:]) != shape[1:]:
+        _refuse("%s: values of shape %s, indices of shape %s, dense_shape %s", what, tuple(values.shape),
+                tuple(indices.shape), shape)
+    if shape[0] < 0:
+        _refuse("%s: dense_shape is %s", what, shape)
+    if torch.cuda.is_current_stream_capturing():
+        _refuse("%s: the size of the result depends on the data: it cannot be captured into a graph", what)
+    out_ids, out_values = _sum_slices(values, indices, shape[0], 1.0)
+    return IndexedSlices(out_values, out_ids, shape)
+
+
+def _sum_slices(values, indices, rows, scale):
+    shape = values.shape[1:]
+    tokens, width = indices.shape[0], 1
+    for d in shape:
+        width *= d
+    flat, stride = _rows_of(values.reshape(tokens, width))
+    indices = indices.contiguous()
+    most = min(tokens, rows)
+    out_ids = torch.empty(most, dtype=indices.dtype, device=values.device)
+    out = torch.empty(most, width, dtype=values.dtype, device=values.device)
+    count = torch.empty(1, dtype=torch.int64, device=values.device)
+    L = step_abi.lib()
+    with _on(values.device) as stream:
+        size = L.step_sum_slices_workspace(tokens, rows, width)
+        ws = _workspace(size, values.device)
+        step_abi.check(L.step_sum_slices(
+            indices.data_ptr(), _IDS[indices.dtype], tokens, flat.data_ptr(), _FLOATS[values.dtype], rows, width, stride,
+            scale, out_ids.data_ptr(), out.data_ptr(), count.data_ptr(), ws.data_ptr(), size, stream), "sum_slices")
+    n = int(count.item())
+    return out_ids[:n], out[:n].reshape((n,) + tuple(shape))
+
+
+class _Embedding(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, ids, weight, scale, sparse):
+        ctx.save_for_backward(ids)
+        ctx.rows, ctx.scale, ctx.sparse = weight.shape[0], scale, sparse
+        ctx.set_materialize_grads(False)
+        return _lookup(ids, weight, scale)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad):
+        if grad is None or not ctx.needs_input_grad[1]:
+            return None, None, None, None
+        ids, = ctx.saved_tensors
+        if not ctx.sparse:
+            return None, _gradient(grad, ids, ctx.rows, ctx.scale), None, None
+        if torch.cuda.is_current_stream_capturing():
+            _refuse("embedding: the size of a sparse gradient depends on the data: it cannot be captured into a graph")
+        index, values = _sum_slices(grad.reshape(ids.numel(), grad.shape[-1]), ids.reshape(-1), ctx.rows, ctx.scale)
+        return None, torch.sparse_coo_tensor(index.long().unsqueeze(0), values, (ctx.rows, grad.shape[-1]),
+                                             is_coalesced=True, check_invariants=False), None, None
+
+
+def embedding(ids, weight, scale=1.0, sparse=False):
+    """Rows of a table by id, times a scale: ids.shape + (width,), in the table's type.
+
+    Arguments:
+        ids: int32 or int64 tensor of any shape. An id outside [0, rows) reads
+             nothing: its row is zero and it has no part in the gradient, so an
+             id of -1 is padding.
+        weight: the table, (rows, width), float32, bfloat16 or float16; rows may be
+                any distance apart (a slice of a larger table).
+        scale: a number every row is multiplied by (sqrt(width), say), in 32 bits
+               before the one rounding to the table's type.
+        sparse: False: weight's gradient is dense (see embedding_gradient). True:
+                it is a sparse tensor with one row per distinct id, which
+                DistributedOptimizer exchanges as an IndexedSlices; its size
+                depends on the data, so that backward pass waits for its stream
+                and cannot be captured into a graph.
+    """
+    what = "embedding"
+    _check_tensor(ids, "ids", _IDS, what)
+    _check_tensor(weight, "weight", _FLOATS, what)
+    _same_device(what, ids, weight)
+    if weight.dim() != 2:
+        _refuse("%s: a table of shape %s; it has two dimensions", what, tuple(weight.shape))
+    scale = float(scale)
+    if torch.is_grad_enabled() and weight.requires_grad:
+        return _Embedding.apply(ids, weight, scale, bool(sparse))
+    return _lookup(ids, weight, scale)

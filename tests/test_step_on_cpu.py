@@ -1,0 +1,99 @@
+"""Checks of the step operators that need no GPU: the C ABI against its
+binding, refusals, the embedding kernels compiled for the CPU under the
+sanitizers (tests/cpp/step_emulation_test.cc), and a scan of the assembly for
+selects on a stale condition code (see test_kernels_on_cpu.py)."""
+import os
+import re
+import shutil
+
+import pytest
+import torch
+
+import mpi_collectives as mpi
+from mpi_collectives import step_abi
+from test_kernels_on_cpu import BUILD, HIP_FLAGS, ROOT, SANITIZERS, SHIM, _clang, _run, kernels_in_scratch, stale_selects
+
+CSRC = os.path.join(ROOT, "tensorflow-allreduce_amd", "csrc")
+EMBEDDING = os.path.join(CSRC, "step_embedding.hip")
+HEADERS = [os.path.join(ROOT, "include", "step_abi.h"), os.path.join(CSRC, "step_common.h")]
+
+
+def test_binding_covers_the_header():
+    text = open(HEADERS[0]).read()
+    text = re.sub(r"/\*.*?\*/", "", text, flags=re.S)
+    declared = sorted(set(re.findall(r"\b(step_\w+)\s*\(", text)))
+    assert sorted(step_abi.EXPORTS) == declared
+    lib = step_abi.lib()
+    assert lib.step_abi_version() == 1
+    for status in range(6):
+        assert lib.step_status_string(status)
+
+
+def test_window_is_the_square_root_and_at_least_64():
+    lib = step_abi.lib()
+    for tokens, window in ((0, 64), (1, 64), (4096, 64), (4097, 128), (16384, 128), (1 << 20, 1024)):
+        assert lib.step_embedding_window(tokens) == window
+
+
+def test_workspace_of_sizes_that_do_not_fit_is_zero():
+    lib = step_abi.lib()
+    assert lib.step_embedding_gradient_workspace(1 << 31, 8, 4) == 0
+    assert lib.step_sum_slices_workspace(8, 1 << 31, 4) == 0
+    assert lib.step_embedding_gradient_workspace(0, 0, 0) > 0
+
+
+@pytest.mark.parametrize("call, words", [
+    (lambda: mpi.embedding([1, 2], torch.zeros(3, 3)), "torch.Tensor"),
+    (lambda: mpi.embedding(torch.zeros(2), torch.zeros(3, 3)), "ids has type"),
+    (lambda: mpi.embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 3)), "GPU kernels only"),
+    (lambda: mpi.embedding_gradient(torch.zeros(2, 3, dtype=torch.float64), torch.zeros(2, dtype=torch.int64), 5), "grad has type"),
+    (lambda: mpi.embedding_gradient(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), 5), "GPU kernels only"),
+    (lambda: mpi.sum_slices(torch.zeros(2, 3)), "IndexedSlices"),
+    (lambda: mpi.sum_slices(mpi.IndexedSlices(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), (5, 3))), "GPU kernels only"),
+])
+def test_refusals_before_any_gpu_work(call, words):
+    with pytest.raises(mpi.InvalidArgumentError, match=re.escape(words)):
+        call()
+
+
+def _emulation(sanitizer):
+    clang = _clang()
+    if clang is None:
+        pytest.skip("no clang++ (the kernels use clang vector extensions)")
+    os.makedirs(BUILD, exist_ok=True)
+    shim = os.path.join(ROOT, "tests", "cpp", "step_wave_shim.h")
+    test = os.path.join(ROOT, "tests", "cpp", "step_emulation_test.cc")
+    flags = ["-std=c++17", "-O1", "-g", "-mf16c", "-fno-omit-frame-pointer", "-pthread", "-I", SHIM,
+             "-I", os.path.join(ROOT, "include")] + SANITIZERS[sanitizer]
+    obj = os.path.join(BUILD, "step_embedding_cpu_%s.o" % sanitizer)
+    exe = os.path.join(BUILD, "step_emulation_test_" + sanitizer)
+    _run([clang, "-x", "c++"] + flags + ["-I", CSRC, "-include", shim, "-c", "-o", obj, EMBEDDING])
+    _run([clang] + flags + ["-o", exe, test, obj])
+    return exe
+
+
+@pytest.mark.parametrize("sanitizer, arguments", [("asan", []), ("tsan", ["brief"])])
+def test_embedding_kernels_under_sanitizers_on_the_cpu(sanitizer, arguments):
+    env = dict(os.environ, TSAN_OPTIONS="halt_on_error=1:report_signal_unsafe=0")
+    out = _run([_emulation(sanitizer)] + arguments, timeout=900, env=env)
+    assert "step emulation: ok" in out, out[-4000:]
+
+
+def _assembly(source):
+    hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
+    if not os.path.exists(hipcc):
+        pytest.skip("hipcc not found")
+    os.makedirs(BUILD, exist_ok=True)
+    asm = os.path.join(BUILD, os.path.basename(source).replace(".hip", "_gfx950.s"))
+    sources = [source, os.path.abspath(__file__)] + HEADERS
+    if not os.path.exists(asm) or os.path.getmtime(asm) < max(os.path.getmtime(f) for f in sources):
+        _run([hipcc] + HIP_FLAGS + ["-I", os.path.join(ROOT, "include"), "-S", "--cuda-device-only", "-o", asm, source])
+    return open(asm).read()
+
+
+def test_embedding_assembly():
+    text = _assembly(EMBEDDING)
+    found = stale_selects(text)
+    assert not found, "scalar selects on a stale condition code: %r" % (found[:5],)
+    kernels = kernels_in_scratch(text, ("lookup_kernel", "sort_one_kernel", "scatter_kernel", "window_kernel", "sum_kernel"))
+    assert kernels["seen"] >= 17 and not kernels["scratch"], kernels
