@@ -26,7 +26,7 @@ constexpr size_t kMostSize = 0x7fffffff;  // tokens, rows, columns: positions an
 
 inline bool is_float(int dtype) { return dtype == STEP_F32 || dtype == STEP_BF16 || dtype == STEP_F16; }
 inline size_t dtype_size(int dtype) { return dtype == STEP_F32 || dtype == STEP_I32 ? 4 : dtype == STEP_I64 ? 8 : 2; }
-inline size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
+__host__ __device__ inline size_t round_up(size_t x, size_t to) { return (x + to - 1) / to * to; }
 
 // ---- element types -------------------------------------------------------------
 // The storage types of the three value types, and their conversions: to 32 bits

@@ -34,6 +34,8 @@ collectives complete at once.
 @@embedding
 @@embedding_gradient
 @@sum_slices
+@@orthogonalize
+@@Muon
 """
 import contextlib
 import os
@@ -45,7 +47,8 @@ from . import _plugin, mpi_ops, ring_abi
 from ._plugin import (FailedPreconditionError, InternalError, InvalidArgumentError,  # noqa: F401
                       NotFoundError, OpError, UnknownError)
 from .mpi_ops import _allreduce, allgather, init, local_rank, rank, size  # noqa: F401
-from .step_ops import IndexedSlices, embedding, embedding_gradient, sum_slices  # noqa: F401
+from .step_ops import (IndexedSlices, Muon, embedding, embedding_gradient, orthogonalize,  # noqa: F401
+                       sum_slices)
 
 _TORCH2RING = {torch.float32: ring_abi.F32, torch.int32: ring_abi.I32, torch.int64: ring_abi.I64}
 

@@ -19,7 +19,15 @@ EXPORTS = (
     "step_abi_version", "step_status_string", "step_last_hip_error",
     "step_embedding_lookup", "step_embedding_window", "step_embedding_gradient_workspace", "step_embedding_gradient",
     "step_sum_slices_workspace", "step_sum_slices",
+    "step_orthogonalize_workspace", "step_orthogonalize", "step_muon",
 )
+
+
+class Matrix(ctypes.Structure):
+    """step_matrix: `count` contiguous matrices of rows x cols."""
+    _fields_ = [("grad", ctypes.c_void_p), ("momentum", ctypes.c_void_p), ("out", ctypes.c_void_p),
+                ("rows", ctypes.c_size_t), ("cols", ctypes.c_size_t), ("count", ctypes.c_size_t),
+                ("rate", ctypes.c_float)]
 
 
 class StepError(RingError):
@@ -44,6 +52,7 @@ def lib():
                 "(the step operators have no CPU fallback)" % LIB_PATH)
         L = ctypes.CDLL(LIB_PATH)
         ci, sz, vp, fl = ctypes.c_int, ctypes.c_size_t, ctypes.c_void_p, ctypes.c_float
+        pm, pf = ctypes.POINTER(Matrix), ctypes.POINTER(fl)
         sig = {
             "step_abi_version": (ci, []),
             "step_status_string": (ctypes.c_char_p, [ci]),
@@ -54,6 +63,9 @@ def lib():
             "step_embedding_gradient": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp, sz, vp]),
             "step_sum_slices_workspace": (sz, [sz, sz, sz]),
             "step_sum_slices": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp, vp, vp, sz, vp]),
+            "step_orthogonalize_workspace": (sz, [pm, sz, ci]),
+            "step_orthogonalize": (ci, [pm, sz, ci, ci, ci, ci, pf, fl, vp, sz, vp]),
+            "step_muon": (ci, [pm, sz, ci, ci, ci, pf, fl, fl, ci, fl, vp, sz, vp]),
         }
         for name in EXPORTS:
             fn = getattr(L, name)          # AttributeError if the symbol is missing

@@ -2,6 +2,7 @@
 binding, refusals, the embedding kernels compiled for the CPU under the
 sanitizers (tests/cpp/step_emulation_test.cc), and a scan of the assembly for
 selects on a stale condition code (see test_kernels_on_cpu.py)."""
+import ctypes
 import os
 import re
 import shutil
@@ -15,6 +16,7 @@ from test_kernels_on_cpu import BUILD, HIP_FLAGS, ROOT, SANITIZERS, SHIM, _clang
 
 CSRC = os.path.join(ROOT, "tensorflow-allreduce_amd", "csrc")
 EMBEDDING = os.path.join(CSRC, "step_embedding.hip")
+ORTHOGONALIZE = os.path.join(CSRC, "step_orthogonalize.hip")
 HEADERS = [os.path.join(ROOT, "include", "step_abi.h"), os.path.join(CSRC, "step_common.h")]
 
 
@@ -48,6 +50,11 @@ def test_workspace_of_sizes_that_do_not_fit_is_zero():
     (lambda: mpi.embedding(torch.zeros(2, dtype=torch.int64), torch.zeros(3, 3)), "GPU kernels only"),
     (lambda: mpi.embedding_gradient(torch.zeros(2, 3, dtype=torch.float64), torch.zeros(2, dtype=torch.int64), 5), "grad has type"),
     (lambda: mpi.embedding_gradient(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), 5), "GPU kernels only"),
+    (lambda: mpi.orthogonalize(torch.zeros(3, 3)), "GPU kernels only"),
+    (lambda: mpi.orthogonalize(torch.zeros(3, 3, dtype=torch.float64)), "update has type"),
+    (lambda: mpi.Muon([torch.nn.Parameter(torch.zeros(3))]), "it takes matrices"),
+    (lambda: mpi.Muon([torch.nn.Parameter(torch.zeros(3, 3))], adjust="x"), "adjust is"),
+    (lambda: mpi.Muon([torch.nn.Parameter(torch.zeros(3, 3))], coefficients=(1, 2)), "coefficients are"),
     (lambda: mpi.sum_slices(torch.zeros(2, 3)), "IndexedSlices"),
     (lambda: mpi.sum_slices(mpi.IndexedSlices(torch.zeros(2, 3), torch.zeros(2, dtype=torch.int64), (5, 3))), "GPU kernels only"),
 ])
@@ -89,6 +96,40 @@ def _assembly(source):
     if not os.path.exists(asm) or os.path.getmtime(asm) < max(os.path.getmtime(f) for f in sources):
         _run([hipcc] + HIP_FLAGS + ["-I", os.path.join(ROOT, "include"), "-S", "--cuda-device-only", "-o", asm, source])
     return open(asm).read()
+
+
+def test_orthogonalize_refuses_on_the_host():
+    """The C entry points' own checks, with pointers that are never followed."""
+    lib = step_abi.lib()
+    M = step_abi.Matrix
+    one = M(4096, 4096, 4096, 100, 200, 3, 0.1)
+    size = lib.step_orthogonalize_workspace(one, 1, 0)
+    assert size > 3 * 128 * 256 * 2 * 4 and lib.step_orthogonalize_workspace(one, 1, 1) > size
+    abc = (ctypes.c_float * 15)()
+
+    def call(m=one, length=1, dtype=0, out=0, steps=5, table=abc, ws=4096, bytes=size):
+        return lib.step_orthogonalize(m, length, dtype, out, 0, steps, table, 0.0, ws, bytes, None)
+
+    assert call(dtype=1) == call(out=2) == 1
+    assert call(steps=-1) == call(steps=65) == call(table=None) == call(ws=None) == call(ws=4097) == call(bytes=size - 1) == 2
+    assert call(m=None) == 2
+    assert call(m=M(None, None, 4096, 100, 200, 3, 0)) == call(m=M(4096, None, None, 100, 200, 3, 0)) == 2
+    assert call(m=M(4096, None, 4096, (1 << 20) + 1, 1, 1, 0)) == call(m=M(4096, None, 4096, 1 << 20, 1 << 20, 1, 0)) == 5
+    assert lib.step_muon(M(4096, None, 4096, 100, 200, 3, 0), 1, 0, 0, 5, abc, 0.0, 0.9, 1, 1.0, 4096, size, None) == 2
+    for empty in (M(None, None, None, 0, 7, 3, 0), M(None, None, None, 7, 0, 3, 0), M(None, None, None, 7, 7, 0, 0)):
+        assert lib.step_orthogonalize_workspace(empty, 1, 0) == 0 and call(m=empty, ws=None, bytes=0) == 0
+    # the workspace of a long list is that of its largest round, not of the whole list
+    many = (M * 500)(*[M(4096, 4096, 4096, 4096, 4096, 1, 0.1) for _ in range(500)])
+    assert lib.step_orthogonalize_workspace(many, 500, 0) < 6 << 30
+    assert lib.step_orthogonalize_workspace(M(4096, None, 4096, 64, 64, 10 ** 7, 0), 1, 0) < 4 << 30
+
+
+def test_orthogonalize_assembly():
+    text = _assembly(ORTHOGONALIZE)
+    found = stale_selects(text)
+    assert not found, "scalar selects on a stale condition code: %r" % (found[:5],)
+    kernels = kernels_in_scratch(text, ("norm_kernel", "first_kernel", "product_kernel", "last_kernel"))
+    assert kernels["seen"] >= 21 and not kernels["scratch"], kernels
 
 
 def test_embedding_assembly():
