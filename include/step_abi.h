@@ -79,13 +79,13 @@ int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* val
 
 /* ---- orthogonalised updates --------------------------------------------------
  * Newton-Schulz steps on the update U of each matrix,
- *   X = U / (|U|_F + eps), then `steps` times  A = X X^T,  X = a X + (b A + c A A) X
+ *   X = U / (|U|_F + eps), then `steps` (1 to 64) times  A = X X^T,  X = a X + (b A + c A A) X
  * (on the transposed matrix if rows > cols; the result is the same), with
  * coefficients[3 k .. 3 k + 2] = a, b, c of step k in host memory.
  *
  * A list of matrices is one call: all of them go through each product in one
- * launch (lists beyond 48 batches or 2^26 elements in several rounds that use
- * the workspace in turn). Matrices are contiguous, `count` of them one behind
+ * launch (lists of more than 64 batches, 32 shapes or 2^26 elements in several
+ * rounds that use the workspace in turn). Matrices are contiguous, `count` of them one behind
  * the other.
  *
  * precise = 0: the products take fp16 operands (the rest of the iterate is kept

@@ -19,6 +19,7 @@
 // a factor of a = 3.4 per step (485 in five), until it is 14 % of the result for
 // an update of rank one, and with it 0.03 to 0.2 % whatever the rank.
 //   SPLIT = false (16-bit results): products of the hi planes.
+//   (The last iterate but one does without: its rounding grows by a once.)
 //   SPLIT = true (float32 results): hi hi + (hi lo + lo hi) / 2048, three products,
 //   22 bits of every operand: about 1e-6 off.
 //
@@ -45,9 +46,11 @@ constexpr float kScaleA = 16384.f;
 constexpr float kScaleB = 1024.f;
 constexpr float kScaleLow = 2048.f;  // hi + lo / 2048: the next 11 bits, away from fp16's smallest numbers
 
-constexpr int kPad = 64;             // and the depth of one stage of a product
-constexpr int kMostSegments = 48;    // of one launch, by value in the kernel's arguments
-constexpr int kNormBlocks = 256;     // partial sums of squares per matrix
+constexpr int kPad = 64;           // and the depth of one stage of a product
+constexpr int kMostItems = 64;     // batches of matrices of one round, by value in the kernels' arguments
+constexpr int kMostGroups = 32;    // and shapes among them
+constexpr int kMostPieces = 1024;  // partial sums of squares per matrix
+constexpr uint64_t kPiece = 8192;  // elements of one, at least
 
 constexpr size_t kMostSide = 1u << 20;
 constexpr size_t kMostElements = 1ull << 33;
@@ -56,15 +59,19 @@ constexpr int kMostSteps = 64;
 // ---- where a matrix keeps its planes -------------------------------------------
 
 struct Planes {
-  uint64_t x_hi, x_lo, y_hi, y_lo, a_hi, a_lo, b_hi, b_lo, norm, bytes;
+  uint64_t norm, x_hi, x_lo, y_hi, y_lo, a_hi, a_lo, b_hi, b_lo, bytes;
   uint64_t y_hi_step, y_lo_step;  // Y has two buffers that take turns; its low plane needs one only if no product reads it
 };
+
+__host__ __device__ inline uint32_t pieces_of(uint64_t size) {
+  return static_cast<uint32_t>(size / kPiece + 1 < kMostPieces ? size / kPiece + 1 : kMostPieces);
+}
 
 __host__ __device__ inline Planes planes_of(uint64_t m, uint64_t n, bool split) {
   Planes p = {};
   uint64_t at = 0;
   const uint64_t mn = m * n * 2, mm = m * m * 2;
-  p.norm = at; at += kNormBlocks * 8;
+  p.norm = at; at += round_up(pieces_of(m * n) * 8, 256);
   p.x_hi = at; at += mn;
   p.y_hi = at; at += 2 * mn;
   p.y_hi_step = mn;
@@ -77,39 +84,53 @@ __host__ __device__ inline Planes planes_of(uint64_t m, uint64_t n, bool split) 
     p.a_lo = at; at += mm;
     p.b_lo = at; at += mm;
   }
-  p.bytes = (at + 255) / 256 * 256;
+  p.bytes = round_up(at, 256);
   return p;
 }
 
-// `count` matrices of one shape, one behind the other in the workspace.
+// Matrices of one shape, one behind the other in the workspace.
 struct Group {
   uint64_t base;
-  uint32_t m, n;        // padded
-  uint32_t first_tile;  // of the launch
-  uint32_t tiles;       // of one matrix
+  uint32_t m, n;          // padded
+  uint32_t first_tile;    // of the launch
+  uint32_t tiles;         // of one matrix
+  uint32_t first_matrix;  // of the round
 };
 struct Groups {
-  Group at[kMostSegments];
+  Group at[kMostGroups];
   int count;
 };
 
-// `count` contiguous matrices of the caller.
+// `count` contiguous updates of the caller.
 struct Segment {
   const void* grad;
   float* momentum;
-  void* out;
   uint64_t base;
   uint32_t rows, cols;
   uint32_t first_tile;
-  uint32_t tiles;       // of one matrix
-  float rate;           // what the orthogonalised update is multiplied by (Muon)
-  int tall;
+  uint32_t tiles;         // of one matrix
 };
 struct Segments {
-  Segment at[kMostSegments];
+  Segment at[kMostItems];
   int count;
 };
 
+// And where their results go.
+struct Target {
+  void* out;
+  uint32_t rows, cols;
+  uint32_t first_tile;    // its first matrix of the round
+  float rate;             // what the orthogonalised update is multiplied by (Muon)
+};
+struct Targets {
+  Target at[kMostItems];
+  int count;
+  int type, muon;
+  float keep;
+};
+struct Nothing {};
+
+// The last entry that begins at or before `tile`.
 template <typename S> __device__ __forceinline__ int find(const S& s, uint32_t tile) {
   int lo = 0, hi = s.count - 1;
   while (lo < hi) {
@@ -132,16 +153,48 @@ struct MomentumRule {
   int nesterov, use;
 };
 
+// `count` (at most four) elements from `p` on, which is aligned to an element only.
+template <typename T> struct Four;
+template <> struct Four<F32> { typedef uint32_t type __attribute__((ext_vector_type(4))); };
+template <> struct Four<BF16> { typedef uint16_t type __attribute__((ext_vector_type(4))); };
+template <> struct Four<F16> { typedef uint16_t type __attribute__((ext_vector_type(4))); };
+template <typename T> struct FourOf {
+  typedef typename Four<T>::type V;
+  typedef V VU __attribute__((aligned(sizeof(T))));
+  struct Array { T at[4]; };
+};
+template <typename T> __device__ __forceinline__ float4v load4(const T* p, uint64_t count) {
+  typename FourOf<T>::Array a = {};
+  if (count >= 4) {
+    a = __builtin_bit_cast(typename FourOf<T>::Array, static_cast<typename FourOf<T>::V>(*reinterpret_cast<const typename FourOf<T>::VU*>(p)));
+  } else {
+    for (int k = 0; k < 3; k++)
+      if (static_cast<uint64_t>(k) < count) a.at[k] = p[k];
+  }
+  return float4v{to_float(a.at[0]), to_float(a.at[1]), to_float(a.at[2]), to_float(a.at[3])};
+}
+template <typename T> __device__ __forceinline__ void store4(T* p, float4v v, uint64_t count) {
+  typename FourOf<T>::Array a;
+  for (int k = 0; k < 4; k++) a.at[k] = from_float<T>(v[k]);
+  if (count >= 4) {
+    *reinterpret_cast<typename FourOf<T>::VU*>(p) = __builtin_bit_cast(typename FourOf<T>::V, a);
+  } else {
+    for (int k = 0; k < 3; k++)
+      if (static_cast<uint64_t>(k) < count) p[k] = a.at[k];
+  }
+}
+
+// Four elements of the update: the gradient, or what the momentum (this step's, written by the norm kernel) makes of it.
 template <typename T>
-__device__ __forceinline__ float update_at(const Segment& s, uint64_t at, const MomentumRule& rule) {
-  const float g = to_float(static_cast<const T*>(s.grad)[at]);
+__device__ __forceinline__ float4v update_at(const Segment& s, uint64_t at, uint64_t count, const MomentumRule& rule) {
+  const float4v g = load4(static_cast<const T*>(s.grad) + at, count);
   if (!rule.use) return g;
-  const float m = s.momentum[at];  // this step's, written by the norm kernel
+  const float4v m = load4(reinterpret_cast<const F32*>(s.momentum) + at, count);
   return rule.nesterov ? g + rule.momentum * m : m;
 }
 
-// One block per piece of a matrix: momentum = mu momentum + grad, and the piece's sum of squares of the update. In 64
-// bits: gradients of 1e-20 have a norm too.
+// One workgroup per piece of a matrix: momentum = mu momentum + grad, and the piece's sum of squares of the update, in 64
+// bits: gradients of 1e-20 have a norm too. Bound by HBM.
 template <typename T>
 __global__ void __launch_bounds__(256) norm_kernel(Segments segments, MomentumRule rule, char* ws, int split) {
   __shared__ double sums[4];
@@ -149,76 +202,94 @@ __global__ void __launch_bounds__(256) norm_kernel(Segments segments, MomentumRu
   const uint32_t matrix = (blockIdx.x - s.first_tile) / s.tiles, piece = (blockIdx.x - s.first_tile) % s.tiles;
   const uint64_t size = static_cast<uint64_t>(s.rows) * s.cols, base = matrix * size;
   const uint64_t length = (size + s.tiles - 1) / s.tiles;
-  const uint64_t end = (piece + 1) * length < size ? (piece + 1) * length : size;
+  const uint64_t begin = piece * length, end = begin + length < size ? begin + length : size;
   double sum = 0;
-  for (uint64_t i = piece * length + threadIdx.x; i < end; i += 256) {
+#pragma unroll 4
+  for (uint64_t i = begin + threadIdx.x * 4; i < end; i += 1024) {
+    float4v u = load4(static_cast<const T*>(s.grad) + base + i, end - i);
     if (rule.use) {
-      const float g = to_float(static_cast<const T*>(s.grad)[base + i]);
-      s.momentum[base + i] = rule.momentum * s.momentum[base + i] + g;
+      const float4v m = rule.momentum * load4(reinterpret_cast<const F32*>(s.momentum) + base + i, end - i) + u;
+      store4(reinterpret_cast<F32*>(s.momentum) + base + i, m, end - i);
+      u = rule.nesterov ? u + rule.momentum * m : m;
     }
-    const double u = update_at<T>(s, base + i, rule);
-    sum += u * u;
+    for (int k = 0; k < 4; k++)
+      if (i + k < end) sum += static_cast<double>(u[k]) * u[k];
   }
   for (int step = 32; step; step /= 2) sum += __shfl_xor(sum, step);
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
   __syncthreads();
   if (threadIdx.x == 0) {
-    const uint64_t m = round_up(s.tall ? s.cols : s.rows, kPad), n = round_up(s.tall ? s.rows : s.cols, kPad);
-    const Planes p = planes_of(m, n, split);
+    const bool tall = s.rows > s.cols;
+    const Planes p = planes_of(round_up(tall ? s.cols : s.rows, kPad), round_up(tall ? s.rows : s.cols, kPad), split);
     reinterpret_cast<double*>(ws + s.base + matrix * p.bytes + p.norm)[piece] = sums[0] + sums[1] + sums[2] + sums[3];
   }
 }
 
-// One block per 64 x 64 tile of U: X_0 by rows and by columns.
+// One workgroup per 64 x 64 tile of U, through LDS: X_0 by rows and by columns. Bound by HBM.
 template <typename T, bool SPLIT>
 __global__ void __launch_bounds__(256) first_kernel(Segments segments, MomentumRule rule, float eps, char* ws) {
   __shared__ float tile[64][65];
   __shared__ double sums[4];
   const Segment& s = segments.at[find(segments, blockIdx.x)];
   const uint32_t matrix = (blockIdx.x - s.first_tile) / s.tiles, t = (blockIdx.x - s.first_tile) % s.tiles;
-  const uint32_t m = static_cast<uint32_t>(round_up(s.tall ? s.cols : s.rows, kPad));
-  const uint32_t n = static_cast<uint32_t>(round_up(s.tall ? s.rows : s.cols, kPad));
+  const bool tall = s.rows > s.cols;
+  const uint32_t m = static_cast<uint32_t>(round_up(tall ? s.cols : s.rows, kPad));
+  const uint32_t n = static_cast<uint32_t>(round_up(tall ? s.rows : s.cols, kPad));
   const Planes p = planes_of(m, n, SPLIT);
   char* at = ws + s.base + matrix * p.bytes;
   const uint64_t size = static_cast<uint64_t>(s.rows) * s.cols;
-  const uint32_t pieces = static_cast<uint32_t>(size / 4096 + 1 < kNormBlocks ? size / 4096 + 1 : kNormBlocks);
-  double sum = threadIdx.x < pieces ? reinterpret_cast<const double*>(at + p.norm)[threadIdx.x] : 0;
+  const uint32_t across = (tall ? m : n) / 64, r0 = t / across * 64, c0 = t % across * 64;
+  const uint32_t row = threadIdx.x / 16, col = threadIdx.x % 16 * 4;
+  float4v u[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    const uint32_t r = r0 + row + k * 16, c = c0 + col;
+    u[k] = r < s.rows && c < s.cols ? update_at<T>(s, matrix * size + static_cast<uint64_t>(r) * s.cols + c, s.cols - c, rule) : float4v{0, 0, 0, 0};
+  }
+  const uint32_t pieces = pieces_of(size);
+  double sum = 0;
+  for (uint32_t k = threadIdx.x; k < pieces; k += 256) sum += reinterpret_cast<const double*>(at + p.norm)[k];
   for (int step = 32; step; step /= 2) sum += __shfl_xor(sum, step);
   if (threadIdx.x % 64 == 0) sums[threadIdx.x / 64] = sum;
   __syncthreads();
   const double scale = kScaleX / (sqrt(sums[0] + sums[1] + sums[2] + sums[3]) + static_cast<double>(eps));
-  // the tile of U
-  const uint32_t across = static_cast<uint32_t>(round_up(s.cols, 64)) / 64;
-  const uint32_t r0 = t / across * 64, c0 = t % across * 64;
-  for (uint32_t k = threadIdx.x; k < 64 * 64; k += 256) {
-    const uint32_t r = r0 + k / 64, c = c0 + k % 64;
-    float u = 0.f;
-    if (r < s.rows && c < s.cols) u = static_cast<float>(update_at<T>(s, matrix * size + static_cast<uint64_t>(r) * s.cols + c, rule) * scale);
-    tile[k / 64][k % 64] = u;
-  }
+#pragma unroll
+  for (int k = 0; k < 4; k++)
+    for (int e = 0; e < 4; e++) tile[row + k * 16][col + e] = static_cast<float>(u[k][e] * scale);
   __syncthreads();
-  // by_rows: the planes whose rows are U's rows; X if U is wide, Y if it is tall
+  // U's rows are X's rows if it is wide, Y's if it is tall
   _Float16* x_hi = reinterpret_cast<_Float16*>(at + p.x_hi);
   _Float16* x_lo = SPLIT ? reinterpret_cast<_Float16*>(at + p.x_lo) : nullptr;
   _Float16* y_hi = reinterpret_cast<_Float16*>(at + p.y_hi);
   _Float16* y_lo = reinterpret_cast<_Float16*>(at + p.y_lo);
-  for (uint32_t k = threadIdx.x; k < 64 * 64; k += 256) {
-    const uint32_t i = k / 64, j = k % 64;
-    _Float16 hi, lo;
-    split_value(tile[i][j], &hi, &lo);
-    const uint64_t by_row = static_cast<uint64_t>(r0 + i) * (s.tall ? m : n) + c0 + j;
-    if (s.tall) { y_hi[by_row] = hi; y_lo[by_row] = lo; }
-    else { x_hi[by_row] = hi; if (SPLIT) x_lo[by_row] = lo; }
-    split_value(tile[j][i], &hi, &lo);
-    const uint64_t by_col = static_cast<uint64_t>(c0 + i) * (s.tall ? n : m) + r0 + j;
-    if (s.tall) { x_hi[by_col] = hi; if (SPLIT) x_lo[by_col] = lo; }
-    else { y_hi[by_col] = hi; y_lo[by_col] = lo; }
+#pragma unroll
+  for (int k = 0; k < 2; k++) {
+    const uint32_t i = threadIdx.x / 8 + k * 32, j = threadIdx.x % 8 * 8;
+    for (int by_col = 0; by_col < 2; by_col++) {
+      half8 hi, lo;
+      for (int e = 0; e < 8; e++) {
+        _Float16 h, l;
+        split_value(by_col ? tile[j + e][i] : tile[i][j + e], &h, &l);
+        hi[e] = h;
+        lo[e] = l;
+      }
+      const bool to_y = tall != (by_col != 0);
+      const uint64_t to = static_cast<uint64_t>((by_col ? c0 : r0) + i) * (to_y ? m : n) + (by_col ? r0 : c0) + j;
+      if (to_y) {
+        *reinterpret_cast<half8*>(y_hi + to) = hi;
+        *reinterpret_cast<half8*>(y_lo + to) = lo;
+      } else {
+        *reinterpret_cast<half8*>(x_hi + to) = hi;
+        if (SPLIT) *reinterpret_cast<half8*>(x_lo + to) = lo;
+      }
+    }
   }
 }
 
 // ---- products -----------------------------------------------------------------------
 
-enum Kind { GRAM, SQUARE, APPLY };
+// A = X X^T; B = b A + c A A; the next X and Y; the last X, to the caller.
+enum Kind { GRAM, SQUARE, APPLY, LAST };
 
 // Moves 16 bytes per lane from global memory into LDS at base + 16 * lane, without registers in between.
 __device__ __forceinline__ void load_to_lds(const void* from, void* base) {
@@ -228,243 +299,389 @@ __device__ __forceinline__ void load_to_lds(const void* from, void* base) {
 }
 
 // A row of a stage is 64 halves: 8 chunks of 16 bytes, whose order depends on the row so that the 16 lanes that read one
-// chunk index of 16 rows touch different banks.
+// chunk index of 16 rows touch different banks (no conflicts measured).
 __device__ __forceinline__ uint32_t chunk_place(uint32_t row, uint32_t chunk) { return chunk ^ ((row >> 1) & 7); }
 
-template <int TM, int TN, int WM, int WN, Kind KIND, bool SPLIT>
-__global__ void __launch_bounds__(WM * WN * 64) product_kernel(Groups groups, char* ws, int from, float a, float b, float c) {
-  constexpr int THREADS = WM * WN * 64;
-  constexpr int FM = TM / WM / 16, FN = TN / WN / 16;
-  constexpr int LOADS = (TM + TN) * 8 / THREADS;     // 16-byte chunks per lane and stage
-  constexpr int STAGE = (TM + TN) * 64;              // halves
-  __shared__ _Float16 lds[2 * STAGE];
-
-  const Group& g = groups.at[find(groups, blockIdx.x)];
-  const uint32_t m = g.m, n = g.n;
-  const uint32_t matrix = (blockIdx.x - g.first_tile) / g.tiles, tile = (blockIdx.x - g.first_tile) % g.tiles;
-  const Planes p = planes_of(m, n, SPLIT);
-  char* at = ws + g.base + matrix * p.bytes;
-
-  uint32_t ti, tj;
-  if (KIND == APPLY) {
-    const uint32_t down = (m + TM - 1) / TM;
-    ti = tile % down;
-    tj = tile / down;
-  } else {                                           // tile i (i + 1) / 2 + j, j <= i
-    ti = static_cast<uint32_t>((sqrtf(8.f * tile + 1.f) - 1.f) * 0.5f);
-    while (ti * (ti + 1) / 2 > tile) ti--;
-    while ((ti + 1) * (ti + 2) / 2 <= tile) ti++;
-    tj = tile - ti * (ti + 1) / 2;
-  }
-  const uint32_t i0 = ti * TM, j0 = tj * TN;
-  const uint32_t depth = KIND == GRAM ? n : m;       // both operands' row length
-  const uint32_t rows_p = m, rows_q = KIND == APPLY ? n : m;
-  const uint64_t y_hi_at = p.y_hi + from * p.y_hi_step, y_lo_at = p.y_lo + from * p.y_lo_step;
-  const uint64_t y_hi_to = p.y_hi + (from ^ 1) * p.y_hi_step, y_lo_to = p.y_lo + (from ^ 1) * p.y_lo_step;
-  const char* p_hi = at + (KIND == GRAM ? p.x_hi : KIND == SQUARE ? p.a_hi : p.b_hi);
-  const char* p_lo = at + (KIND == GRAM ? p.x_lo : KIND == SQUARE ? p.a_lo : p.b_lo);
-  const char* q_hi = KIND == APPLY ? at + y_hi_at : p_hi;
-  const char* q_lo = KIND == APPLY ? at + y_lo_at : p_lo;
-
-  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-  // what this lane loads: one chunk of each of LOADS rows; rows behind the matrix repeat its last one
-  uint32_t offset[LOADS];
-  for (int k = 0; k < LOADS; k++) {
-    const uint32_t chunk = k * THREADS + threadIdx.x, row = chunk / 8;
-    const bool second = row >= TM;
-    uint32_t r = second ? j0 + row - TM : i0 + row;
-    const uint32_t last = (second ? rows_q : rows_p) - 1;
-    r = r < last ? r : last;
-    offset[k] = chunk_place(row, chunk % 8) * 16;
-    // rows times their length may pass 32 bits: kept in units of 16 bytes
-    offset[k] = r * (depth / 8) + offset[k] / 16;
-  }
-  const uint32_t steps = depth / 64;
-  const uint32_t total = SPLIT ? 3 * steps : steps;
-  auto issue = [&](uint32_t step) {
-    const uint32_t part = SPLIT ? step / steps : 2, k0 = SPLIT ? step % steps : step;
-    const char* from_p = part == 1 ? p_lo : p_hi;    // hi lo, lo hi, hi hi
-    const char* from_q = part == 0 ? q_lo : q_hi;
-    _Float16* to = lds + (step & 1) * STAGE + wave * 64 * 8;
-    for (int k = 0; k < LOADS; k++) {
-      const bool second = k * THREADS / 8 >= TM;
-      load_to_lds((second ? from_q : from_p) + (static_cast<uint64_t>(offset[k]) + k0 * 8) * 16, to + k * THREADS * 8);
-    }
-  };
-  static_assert(TM * 8 % THREADS == 0, "a load belongs to one operand");
-
-  const uint32_t wi = wave / WN * (TM / WM), wj = wave % WN * (TN / WN);
-  float4v acc[FM][FN] = {};
-  issue(0);
-  for (uint32_t step = 0; step < total; step++) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (step + 1 < total) issue(step + 1);
-    if (SPLIT && step == 2 * steps) {
-      for (int x = 0; x < FM; x++)
-        for (int y = 0; y < FN; y++) acc[x][y] *= 1.f / kScaleLow;
-    }
-    const _Float16* stage = lds + (step & 1) * STAGE;
-    for (int s = 0; s < 2; s++) {
-      half8 fp[FM], fq[FN];
-      const uint32_t chunk = s * 4 + lane / 16;
-      for (int x = 0; x < FM; x++) {
-        const uint32_t row = wi + x * 16 + lane % 16;
-        fp[x] = *reinterpret_cast<const half8*>(stage + row * 64 + chunk_place(row, chunk) * 8);
-      }
-      for (int y = 0; y < FN; y++) {
-        const uint32_t row = TM + wj + y * 16 + lane % 16;
-        fq[y] = *reinterpret_cast<const half8*>(stage + row * 64 + chunk_place(row, chunk) * 8);
-      }
-      for (int x = 0; x < FM; x++)
-        for (int y = 0; y < FN; y++) acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[x], fq[y], acc[x][y], 0, 0, 0);
-    }
-  }
-
-  // a lane holds rows 4 (lane / 16) + 0..3 and column lane % 16 of every 16 x 16 piece
-  for (int x = 0; x < FM; x++) {
-    const uint32_t i = i0 + wi + x * 16 + lane / 16 * 4;
-    if (i >= m) continue;
-    for (int y = 0; y < FN; y++) {
-      const uint32_t j = j0 + wj + y * 16 + lane % 16;
-      if (j >= rows_q) continue;
-      half4 hi, lo;
-      if (KIND == APPLY) {
-        const uint64_t by_col = static_cast<uint64_t>(j) * m + i;
-        const half4 old_hi = *reinterpret_cast<const half4*>(at + y_hi_at + by_col * 2);
-        const half4 old_lo = *reinterpret_cast<const half4*>(at + y_lo_at + by_col * 2);
-        for (int e = 0; e < 4; e++) {
-          const float v = a * (static_cast<float>(old_hi[e]) + static_cast<float>(old_lo[e]) * (1.f / kScaleLow)) + acc[x][y][e] * (1.f / kScaleB);
-          _Float16 h, l;
-          split_value(v, &h, &l);
-          hi[e] = h;
-          lo[e] = l;
-        }
-        *reinterpret_cast<half4*>(at + y_hi_to + by_col * 2) = hi;
-        *reinterpret_cast<half4*>(at + y_lo_to + by_col * 2) = lo;
-        for (int e = 0; e < 4; e++) {
-          const uint64_t by_row = static_cast<uint64_t>(i + e) * n + j;
-          reinterpret_cast<_Float16*>(at + p.x_hi)[by_row] = hi[e];
-          if (SPLIT) reinterpret_cast<_Float16*>(at + p.x_lo)[by_row] = lo[e];
-        }
-      } else {
-        const uint64_t to_hi = KIND == GRAM ? p.a_hi : p.b_hi, to_lo = KIND == GRAM ? p.a_lo : p.b_lo;
-        const uint64_t by_col = static_cast<uint64_t>(j) * m + i;
-        half4 a_hi = {}, a_lo = {};
-        if (KIND == SQUARE) {
-          a_hi = *reinterpret_cast<const half4*>(at + p.a_hi + by_col * 2);
-          if (SPLIT) a_lo = *reinterpret_cast<const half4*>(at + p.a_lo + by_col * 2);
-        }
-        for (int e = 0; e < 4; e++) {
-          float v;
-          if (KIND == GRAM) {
-            v = acc[x][y][e] * (kScaleA / (kScaleX * kScaleX));
-          } else {
-            const float old = static_cast<float>(a_hi[e]) + (SPLIT ? static_cast<float>(a_lo[e]) * (1.f / kScaleLow) : 0.f);
-            v = b * (kScaleB / kScaleA) * old + c * (kScaleB / kScaleA / kScaleA) * acc[x][y][e];
-          }
-          _Float16 h, l;
-          split_value(v, &h, &l);
-          hi[e] = h;
-          lo[e] = l;
-        }
-        // the tile and, off the diagonal, its mirror image
-        for (int e = 0; e < 4; e++) {
-          const uint64_t by_row = static_cast<uint64_t>(i + e) * m + j;
-          reinterpret_cast<_Float16*>(at + to_hi)[by_row] = hi[e];
-          if (SPLIT) reinterpret_cast<_Float16*>(at + to_lo)[by_row] = lo[e];
-        }
-        if (ti != tj) {
-          *reinterpret_cast<half4*>(at + to_hi + by_col * 2) = hi;
-          if (SPLIT) *reinterpret_cast<half4*>(at + to_lo + by_col * 2) = lo;
-        }
-      }
-    }
+// Asks the compiler to mix the LDS reads and global loads of a half step among its products instead of putting them first.
+template <int READS, int PRODUCTS, int LOADS> __device__ __forceinline__ void interleave() {
+  constexpr int EACH = PRODUCTS / (READS + LOADS) > 0 ? PRODUCTS / (READS + LOADS) : 1;
+#pragma unroll
+  for (int k = 0; k < READS + LOADS; k++) {
+    __builtin_amdgcn_sched_group_barrier(0x008, EACH, 0);
+    if (k % 2 == 0 && k / 2 < LOADS) __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+    else __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
   }
 }
 
-// ---- the result -----------------------------------------------------------------------
+template <int N> __device__ __forceinline__ void wait_loads() {
+  asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
-// One block per 64 x 64 tile of the result: out = X (orthogonalize) or out = keep out - rate X (Muon).
-template <typename T, bool SPLIT>
-__global__ void __launch_bounds__(256) last_kernel(Segments segments, int from, int muon, float keep, const char* ws) {
-  __shared__ float tile[64][65];
-  const Segment& s = segments.at[find(segments, blockIdx.x)];
-  const uint32_t matrix = (blockIdx.x - s.first_tile) / s.tiles, t = (blockIdx.x - s.first_tile) % s.tiles;
-  const uint32_t m = static_cast<uint32_t>(round_up(s.tall ? s.cols : s.rows, kPad));
-  const uint32_t n = static_cast<uint32_t>(round_up(s.tall ? s.rows : s.cols, kPad));
-  const Planes p = planes_of(m, n, SPLIT);
-  const char* at = ws + s.base + matrix * p.bytes;
-  const _Float16* y_hi = reinterpret_cast<const _Float16*>(at + p.y_hi + from * p.y_hi_step);
-  const _Float16* y_lo = reinterpret_cast<const _Float16*>(at + p.y_lo + from * p.y_lo_step);
-  const uint32_t across = static_cast<uint32_t>(round_up(s.cols, 64)) / 64;
-  const uint32_t r0 = t / across * 64, c0 = t % across * 64;
-  // Y's rows are the result's rows if it is tall, else its columns
-  for (uint32_t k = threadIdx.x; k < 64 * 64; k += 256) {
-    const uint32_t i = k / 64, j = k % 64;
-    const uint64_t from_at = static_cast<uint64_t>((s.tall ? r0 : c0) + i) * m + (s.tall ? c0 : r0) + j;
-    const float v = (static_cast<float>(y_hi[from_at]) + static_cast<float>(y_lo[from_at]) * (1.f / kScaleLow)) * (1.f / kScaleX);
-    if (s.tall) tile[i][j] = v;
-    else tile[j][i] = v;
+// Four lanes side by side hold four rows of one column each; afterwards four columns of one row each.
+__device__ __forceinline__ half4 transpose4(half4 v) {
+  typedef uint32_t pair __attribute__((ext_vector_type(2)));
+  pair r = __builtin_bit_cast(pair, v);
+  const uint32_t lane = threadIdx.x;
+  // with the lane next to it: 2 x 2 blocks
+  const uint32_t o0 = __builtin_amdgcn_mov_dpp(r.x, 0xb1, 0xf, 0xf, true), o1 = __builtin_amdgcn_mov_dpp(r.y, 0xb1, 0xf, 0xf, true);
+  // even: (mine[0], theirs[0]); odd: (theirs[1], mine[1])
+  const uint32_t even0 = __builtin_amdgcn_perm(o0, r.x, 0x05040100), even1 = __builtin_amdgcn_perm(o1, r.y, 0x05040100);
+  const uint32_t odd0 = __builtin_amdgcn_perm(r.x, o0, 0x07060302), odd1 = __builtin_amdgcn_perm(r.y, o1, 0x07060302);
+  r.x = lane & 1 ? odd0 : even0;
+  r.y = lane & 1 ? odd1 : even1;
+  // with the lane two further on: the blocks off the diagonal change places
+  const uint32_t p0 = __builtin_amdgcn_mov_dpp(r.x, 0x4e, 0xf, 0xf, true), p1 = __builtin_amdgcn_mov_dpp(r.y, 0x4e, 0xf, 0xf, true);
+  pair out;
+  out.x = lane & 2 ? p1 : r.x;
+  out.y = lane & 2 ? r.y : p0;
+  return __builtin_bit_cast(half4, out);
+}
+
+__device__ __forceinline__ float4v transpose4(float4v v) {
+  const uint32_t lane = threadIdx.x;
+  auto next = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0xb1, 0xf, 0xf, true)); };
+  auto after_next = [](float x) { return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), 0x4e, 0xf, 0xf, true)); };
+  const float s0 = next(lane & 1 ? v[0] : v[1]), s1 = next(lane & 1 ? v[2] : v[3]);
+  if (lane & 1) { v[0] = s0; v[2] = s1; }
+  else { v[1] = s0; v[3] = s1; }
+  const float t0 = after_next(lane & 2 ? v[0] : v[2]), t1 = after_next(lane & 2 ? v[1] : v[3]);
+  if (lane & 2) { v[0] = t0; v[1] = t1; }
+  else { v[2] = t0; v[3] = t1; }
+  return v;
+}
+
+// Tile t of the triangle of a square of `down` x `down` tiles, on and below the diagonal, in blocks of 4 x 4 tiles: what
+// runs at the same time shares rows.
+__device__ __forceinline__ void triangle_tile(uint32_t t, uint32_t down, uint32_t* ti, uint32_t* tj) {
+  uint32_t block = static_cast<uint32_t>((sqrtf(8.f * t + 1.f) - 1.f) * 0.125f);
+  while (block && 2 * block * (4 * block + 1) > t) block--;
+  while (2 * (block + 1) * (4 * block + 5) <= t) block++;
+  t -= 2 * block * (4 * block + 1);                      // 4 block (4 block + 1) / 2 tiles above
+  const uint32_t high = down - 4 * block < 4 ? down - 4 * block : 4;
+  const uint32_t across = t / (high * 4);
+  if (across < block) {
+    t -= across * high * 4;
+    *ti = 4 * block + t % high;
+    *tj = 4 * across + t / high;
+  } else {
+    t -= block * high * 4;
+    uint32_t i = 0;
+    while ((i + 1) * (i + 2) / 2 <= t) i++;
+    *ti = 4 * block + i;
+    *tj = 4 * block + t - i * (i + 1) / 2;
   }
-  __syncthreads();
-  const uint64_t size = static_cast<uint64_t>(s.rows) * s.cols;
-  T* out = static_cast<T*>(s.out) + matrix * size;
-  for (uint32_t k = threadIdx.x; k < 64 * 64; k += 256) {
-    const uint32_t r = r0 + k / 64, c = c0 + k % 64;
-    if (r >= s.rows || c >= s.cols) continue;
-    const uint64_t to = static_cast<uint64_t>(r) * s.cols + c;
-    const float v = tile[k / 64][k % 64];
-    out[to] = from_float<T>(muon ? keep * to_float(out[to]) - s.rate * v : v);
+}
+
+// Tile t of down x across, in strips of eight rows of tiles.
+__device__ __forceinline__ void square_tile(uint32_t t, uint32_t down, uint32_t across, uint32_t* ti, uint32_t* tj) {
+  const uint32_t strip = t / (8 * across), high = down - 8 * strip < 8 ? down - 8 * strip : 8;
+  t -= strip * 8 * across;
+  *ti = strip * 8 + t % high;
+  *tj = t / high;
+}
+
+// One product of a step for all matrices of a launch. A workgroup makes a SIDE x SIDE tile with KS groups of WM x WN waves,
+// which take the stages of 64 halves of depth in turn and add their sums up in LDS at the end (tiles of 64: a matrix
+// has few, and its depth is what takes the time).
+template <int SIDE, int WM, int WN, int KS, int STAGES, Kind KIND, bool SPLIT>
+__global__ void __launch_bounds__(KS * WM * WN * 64, 2)
+    product_kernel(Groups groups, std::conditional_t<KIND == LAST, Targets, Nothing> targets, char* ws, int from, int low_in,
+                   int low_out, float a, float b, float c) {
+  constexpr bool FROM_Y = KIND == APPLY || KIND == LAST;
+  constexpr int PLANES = SPLIT ? 2 : 1;
+  constexpr int THREADS = WM * WN * 64;                     // of a group
+  constexpr int FM = SIDE / WM / 16, FN = SIDE / WN / 16;   // 16 x 16 pieces of a wave
+  constexpr int SUB = PLANES * 2 * SIDE * 64;               // halves of one group's stage: hi rows of both operands, lo rows
+  constexpr int LOADS = PLANES * 2 * SIDE * 8 / THREADS;    // 16-byte chunks per lane and stage
+  constexpr int PER_OPERAND = SIDE * 8 / THREADS;
+  static_assert(SIDE * 8 % THREADS == 0, "a load belongs to one operand");
+  static_assert(KS == 1 || (KS == 2 && FN % 2 == 0), "");
+  constexpr int EN = FN / KS;                               // pieces across that a wave finishes
+  constexpr int STAGED = STAGES * KS * SUB, SUMS = KS == 1 ? 0 : KS * SIDE * SIDE * 2;
+  __shared__ _Float16 lds[STAGED > SUMS ? STAGED : SUMS];
+
+  // Workgroups are dealt to the eight chiplets in turn: give each chiplet, and its cache, neighbouring tiles.
+  const uint32_t share = gridDim.x / 8, spare = gridDim.x % 8, chiplet = blockIdx.x % 8;
+  const uint32_t of_all = chiplet * share + (chiplet < spare ? chiplet : spare) + blockIdx.x / 8;
+  const Group& g = groups.at[find(groups, of_all)];
+  const uint32_t m = g.m, n = g.n, matrix = (of_all - g.first_tile) / g.tiles, tile = (of_all - g.first_tile) % g.tiles;
+  const Planes p = planes_of(m, n, SPLIT);
+  char* at = ws + g.base + matrix * p.bytes;
+  uint32_t ti, tj;
+  if (FROM_Y) square_tile(tile, (m + SIDE - 1) / SIDE, (n + SIDE - 1) / SIDE, &ti, &tj);
+  else triangle_tile(tile, (m + SIDE - 1) / SIDE, &ti, &tj);
+  const uint32_t i0 = ti * SIDE, j0 = tj * SIDE, rows_q = FROM_Y ? n : m;
+  const uint32_t depth = KIND == GRAM ? n : m, last = depth / 64;
+
+  const uint32_t lane = threadIdx.x % 64, wave = __builtin_amdgcn_readfirstlane(threadIdx.x / 64);
+  const uint32_t mine = wave / (WM * WN), place = wave % (WM * WN);  // the wave's group, and its place there
+  const uint32_t wi = place / WN * (SIDE / WM), wj = place % WN * (SIDE / WN);
+
+  // What this lane loads: a chunk of each of PER_OPERAND rows of either operand, as bytes from the tile's first row (at
+  // most 256 rows of 2^20 columns); rows behind the matrix repeat its last one.
+  uint32_t offset[2 * PER_OPERAND];
+#pragma unroll
+  for (int k = 0; k < 2 * PER_OPERAND; k++) {
+    const uint32_t chunk = k * THREADS + threadIdx.x % THREADS, row = chunk / 8;
+    const bool second = k >= PER_OPERAND;
+    const uint32_t r = second ? row - SIDE : row, end = second ? rows_q - j0 - 1 : m - i0 - 1;
+    offset[k] = ((r < end ? r : end) * (depth / 8) + chunk_place(row, chunk % 8)) * 16;
+  }
+  const uint64_t row_p = static_cast<uint64_t>(i0) * depth * 2, row_q = static_cast<uint64_t>(j0) * depth * 2;
+  const uint64_t y_hi = p.y_hi + from * p.y_hi_step, y_lo = p.y_lo + from * p.y_lo_step;
+  const char* operand[4] = {at + row_p + (KIND == GRAM ? p.x_hi : KIND == SQUARE ? p.a_hi : p.b_hi),
+                            at + row_q + (KIND == GRAM ? p.x_hi : KIND == SQUARE ? p.a_hi : y_hi),
+                            at + row_p + (KIND == GRAM ? p.x_lo : KIND == SQUARE ? p.a_lo : p.b_lo),
+                            at + row_q + (KIND == GRAM ? p.x_lo : KIND == SQUARE ? p.a_lo : y_lo)};
+  // the stages that begin at `step`, one for each group (behind the end: the last one again, which nobody multiplies)
+  auto issue = [&](uint32_t step, uint32_t buffer) {
+    step = KS == 1 || step + mine < last ? step + mine : last - 1;
+    _Float16* to = lds + (buffer * KS + mine) * SUB + place * 64 * 8;
+#pragma unroll
+    for (int k = 0; k < LOADS; k++)
+      load_to_lds(operand[k / PER_OPERAND] + step * 128ull + offset[k % (2 * PER_OPERAND)], to + k * THREADS * 8);
+  };
+
+  float4v acc[FM][FN] = {}, low[SPLIT ? FM : 1][SPLIT ? FN : 1] = {};
+  // Fragments are read a half stage ahead of the products that use them, so that LDS and the matrix cores work at the
+  // same time also where a SIMD has one wave.
+  half8 fp[2][PLANES][FM], fq[2][PLANES][FN];
+  auto read = [&](uint32_t buffer, int s) {
+    const _Float16* stage = lds + (buffer * KS + mine) * SUB;
+    const uint32_t chunk = s * 4 + lane / 16;
+#pragma unroll
+    for (int h = 0; h < PLANES; h++) {
+#pragma unroll
+      for (int x = 0; x < FM; x++) {
+        const uint32_t row = wi + x * 16 + lane % 16;
+        fp[s][h][x] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + row) * 64 + chunk_place(row, chunk) * 8);
+      }
+#pragma unroll
+      for (int y = 0; y < FN; y++) {
+        const uint32_t row = SIDE + wj + y * 16 + lane % 16;
+        fq[s][h][y] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + row) * 64 + chunk_place(row, chunk) * 8);
+      }
+    }
+  };
+  auto multiply = [&](int s) {
+#pragma unroll
+    for (int x = 0; x < FM; x++)
+#pragma unroll
+      for (int y = 0; y < FN; y++) {
+        acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[s][0][x], fq[s][0][y], acc[x][y], 0, 0, 0);
+        if constexpr (SPLIT) {
+          low[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[s][0][x], fq[s][1][y], low[x][y], 0, 0, 0);
+          low[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[s][1][x], fq[s][0][y], low[x][y], 0, 0, 0);
+        }
+      }
+  };
+  constexpr int READS = PLANES * (FM + FN), PRODUCTS = FM * FN * (SPLIT ? 3 : 1);
+#pragma unroll
+  for (int k = 0; k < STAGES; k++)
+    if (static_cast<uint32_t>(k * KS) < last) issue(k * KS, k);
+  // the first stage has landed when at most the later ones' loads are under way
+  if ((STAGES - 1) * KS < last) wait_loads<(STAGES - 1) * LOADS>();
+  else wait_loads<0>();
+  read(0, 0);
+  uint32_t step = 0, buffer = 0;
+  auto after = [](uint32_t buffer) { return buffer + 1 == STAGES ? 0 : buffer + 1; };
+  for (; step + STAGES * KS < last; step += KS, buffer = after(buffer)) {
+    read(buffer, 1);
+    multiply(0);
+    interleave<READS, PRODUCTS, 0>();
+    // behind the barrier the next stage has landed, and every wave has read all of this one, which the loads overwrite
+    wait_loads<(STAGES - 2) * LOADS>();
+    issue(step + STAGES * KS, buffer);
+    read(after(buffer), 0);
+    multiply(1);
+    interleave<READS, PRODUCTS, LOADS>();
+  }
+  for (; step < last; step += KS, buffer = after(buffer)) {
+    const bool busy = KS == 1 || step + mine < last;
+    read(buffer, 1);
+    if (busy) multiply(0);
+    wait_loads<0>();
+    if (step + KS < last) read(after(buffer), 0);
+    if (busy) multiply(1);
+  }
+  if constexpr (SPLIT) {
+#pragma unroll
+    for (int x = 0; x < FM; x++)
+#pragma unroll
+      for (int y = 0; y < FN; y++) acc[x][y] += low[x][y] * (1.f / kScaleLow);
+  }
+
+  // the groups' sums, in their order; each goes on with its share of the pieces of a place in the tile
+  const uint32_t ey = mine * EN;
+  float4v sum[FM][EN];
+  if constexpr (KS == 1) {
+#pragma unroll
+    for (int x = 0; x < FM; x++)
+#pragma unroll
+      for (int y = 0; y < EN; y++) sum[x][y] = acc[x][y];
+  } else {
+    constexpr int GROUP = WM * WN * FM * FN * 64;
+    float4v* sums = reinterpret_cast<float4v*>(lds) + place * (FM * FN * 64) + lane;
+    wait_loads<0>();
+#pragma unroll
+    for (int x = 0; x < FM; x++)
+#pragma unroll
+      for (int y = 0; y < FN; y++) sums[mine * GROUP + (x * FN + y) * 64] = acc[x][y];
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < FM; x++)
+#pragma unroll
+      for (int y = 0; y < EN; y++) {
+        sum[x][y] = sums[(x * FN + y + ey) * 64];
+#pragma unroll
+        for (int k = 1; k < KS; k++) sum[x][y] += sums[k * GROUP + (x * FN + y + ey) * 64];
+      }
+  }
+
+  // A lane holds rows 4 (lane / 16) + 0..3 and column lane % 16 of every 16 x 16 piece: 8 bytes of what is stored by
+  // columns. Exchanged among four lanes it is 8 bytes of what is stored by rows. Addresses: the wave's corner, the same
+  // for all its lanes, then 32 bits for a lane's place in it.
+  const uint64_t old_hi_at = FROM_Y ? y_hi : p.a_hi, old_lo_at = FROM_Y ? y_lo : p.a_lo;
+  const uint64_t col_hi_at = KIND == APPLY ? p.y_hi + (from ^ 1) * p.y_hi_step : KIND == GRAM ? p.a_hi : p.b_hi;
+  const uint64_t col_lo_at = KIND == APPLY ? p.y_lo + (from ^ 1) * p.y_lo_step : KIND == GRAM ? p.a_lo : p.b_lo;
+  const uint64_t row_hi_at = KIND == APPLY ? p.x_hi : col_hi_at, row_lo_at = KIND == APPLY ? p.x_lo : col_lo_at;
+  const uint32_t row_length = FROM_Y ? n : m;
+  const uint64_t corner_i = i0 + wi, corner_j = j0 + wj + ey * 16;
+  const uint64_t col_corner = (corner_j * m + corner_i) * 2, row_corner = (corner_i * row_length + corner_j) * 2;
+  const uint32_t col_lane = (lane % 16 * m + lane / 16 * 4) * 2;
+  const uint32_t row_lane = ((lane / 16 * 4 + lane % 4) * row_length + lane % 16 / 4 * 4) * 2;
+  // The linear term's operand is fetched some rows of pieces ahead of its use: the stores may not pass the loads.
+  constexpr int AHEAD = FM < 4 ? FM : 4;
+  const bool with_low = KIND != GRAM && (SPLIT || (FROM_Y && low_in));
+  half4 old_hi[AHEAD][EN], old_lo[AHEAD][EN];
+  auto fetch = [&](int x) {
+    if (KIND == GRAM || corner_i + x * 16 >= m) return;
+#pragma unroll
+    for (int y = 0; y < EN; y++) {
+      if (corner_j + y * 16 >= rows_q) break;
+      const char* from_col = at + col_corner + (static_cast<uint64_t>(y) * 16 * m + x * 16) * 2;
+      old_hi[x % AHEAD][y] = *reinterpret_cast<const half4*>(from_col + old_hi_at + col_lane);
+      if (with_low) old_lo[x % AHEAD][y] = *reinterpret_cast<const half4*>(from_col + old_lo_at + col_lane);
+    }
+  };
+  Target t = {};
+  bool tall = false, muon = false;
+  float keep = 0.f;
+  if constexpr (KIND == LAST) {
+    const uint32_t number = g.first_matrix + matrix;
+    t = targets.at[find(targets, number)];
+    const uint64_t skip = static_cast<uint64_t>(number - t.first_tile) * t.rows * t.cols;
+    t.out = static_cast<char*>(t.out) + skip * (targets.type == STEP_F32 ? 4 : 2);
+    tall = t.rows > t.cols;
+    muon = targets.muon;
+    keep = targets.keep;
+  }
+  auto finish = [&](auto type) {
+    typedef decltype(type) T;
+#pragma unroll
+    for (int x = 0; x < AHEAD - 1; x++) fetch(x);
+#pragma unroll
+    for (int x = 0; x < FM; x++) {
+      if (x + AHEAD - 1 < FM) fetch(x + AHEAD - 1);
+      if (corner_i + x * 16 >= m) break;
+#pragma unroll
+      for (int y = 0; y < EN; y++) {
+        if (corner_j + y * 16 >= rows_q) break;
+        float4v v;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          if (KIND == GRAM) {
+            v[e] = sum[x][y][e] * (kScaleA / (kScaleX * kScaleX));
+          } else {
+            float old = static_cast<float>(old_hi[x % AHEAD][y][e]);
+            if (with_low) old += static_cast<float>(old_lo[x % AHEAD][y][e]) * (1.f / kScaleLow);
+            v[e] = FROM_Y ? a * old + sum[x][y][e] * (1.f / kScaleB)
+                          : b * (kScaleB / kScaleA) * old + c * (kScaleB / kScaleA / kScaleA) * sum[x][y][e];
+          }
+        }
+        if constexpr (KIND == LAST) {
+          v = v * (1.f / kScaleX);
+          if (!tall) v = transpose4(v);
+          const uint64_t i = corner_i + x * 16 + lane / 16 * 4, j = corner_j + y * 16 + lane % 16;
+          const uint64_t r = tall ? j : i + lane % 4, col = tall ? i : j / 4 * 4;
+          if (r < t.rows && col < t.cols) {
+            T* to = static_cast<T*>(t.out) + r * t.cols + col;
+            if (muon) v = keep * load4(to, t.cols - col) - t.rate * v;
+            store4(to, v, t.cols - col);
+          }
+        } else {
+          half4 hi, lo;
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            _Float16 h, l;
+            split_value(v[e], &h, &l);
+            hi[e] = h;
+            lo[e] = l;
+          }
+          char* to_col = at + col_corner + (static_cast<uint64_t>(y) * 16 * m + x * 16) * 2;
+          char* to_row = at + row_corner + (static_cast<uint64_t>(x) * 16 * row_length + y * 16) * 2;
+          if (KIND == APPLY || ti != tj) {                 // Y; the mirror image of a tile off the diagonal
+            *reinterpret_cast<half4*>(to_col + col_hi_at + col_lane) = hi;
+            if (SPLIT || (KIND == APPLY && low_out)) *reinterpret_cast<half4*>(to_col + col_lo_at + col_lane) = lo;
+          }
+          *reinterpret_cast<half4*>(to_row + row_hi_at + row_lane) = transpose4(hi);
+          if (SPLIT) *reinterpret_cast<half4*>(to_row + row_lo_at + row_lane) = transpose4(lo);
+        }
+      }
+    }
+  };
+  if constexpr (KIND == LAST) {
+    if (targets.type == STEP_F32) finish(F32());
+    else if (targets.type == STEP_BF16) finish(BF16());
+    else finish(F16());
+  } else {
+    finish(F32());
   }
 }
 
 // ---- host side -----------------------------------------------------------------------
 
-// What one run through the phases takes: segments in the order of their padded shapes, the groups they make.
-struct Chunk {
-  Segments segments;
-  Groups groups;
-  uint64_t bytes;
-};
-
-// Matrices of one chunk, beyond which more of them fill the GPU no better and only ask for more workspace.
-constexpr uint64_t kChunkElements = 1ull << 26;
+// Elements of one round, beyond which more matrices fill the GPU no better and only ask for more workspace.
+constexpr uint64_t kRoundElements = 1ull << 26;
 
 struct Item {
   size_t matrix, first, count;  // matrices [first, first + count) of the caller's batch `matrix`
   uint32_t m, n;
 };
 
-// Cuts the caller's list into chunks; visit(items, number of items) for each. No memory: items by value.
+// Cuts the caller's list into rounds, their items in the order of their padded shapes; visit(items, their number) for each.
 template <typename Visit>
-int for_chunks(const step_matrix* list, size_t length, const Visit& visit) {
-  Item items[kMostSegments];
-  int used = 0;
+int for_rounds(const step_matrix* list, size_t length, const Visit& visit) {
+  Item items[kMostItems];
+  int used = 0, shapes = 0;
   uint64_t elements = 0;
   auto flush = [&]() {
     if (!used) return static_cast<int>(STEP_OK);
-    std::stable_sort(items, items + used, [](const Item& x, const Item& y) { return x.m != y.m ? x.m < y.m : x.n < y.n; });
-    const int rc = visit(items, used);
-    used = 0;
+    std::stable_sort(items, items + used, [](const Item& x, const Item& y) { return x.m != y.m ? x.m > y.m : x.n > y.n; });
+    const int rc = visit(static_cast<const Item*>(items), used);
+    used = shapes = 0;
     elements = 0;
     return rc;
   };
   for (size_t k = 0; k < length; k++) {
     const size_t rows = list[k].rows, cols = list[k].cols;
+    if (rows == 0 || cols == 0) continue;
     const uint32_t m = static_cast<uint32_t>(round_up(std::min(rows, cols), kPad));
     const uint32_t n = static_cast<uint32_t>(round_up(std::max(rows, cols), kPad));
-    if (rows == 0 || cols == 0) continue;
     const uint64_t one = static_cast<uint64_t>(m) * n;
     size_t first = 0;
     while (first < list[k].count) {
-      const uint64_t room = elements < kChunkElements ? (kChunkElements - elements) / one : 0;
-      if (used == kMostSegments || (room == 0 && used)) {
+      bool known = false;
+      for (int j = 0; j < used && !known; j++) known = items[j].m == m && items[j].n == n;
+      const uint64_t room = elements < kRoundElements ? (kRoundElements - elements) / one : 0;
+      if (used == kMostItems || (!known && shapes == kMostGroups) || (room == 0 && used)) {
         const int rc = flush();
         if (rc != STEP_OK) return rc;
         continue;
       }
       const size_t take = static_cast<size_t>(std::min<uint64_t>(list[k].count - first, std::max<uint64_t>(room, 1)));
       items[used++] = {k, first, take, m, n};
+      shapes += known ? 0 : 1;
       elements += take * one;
       first += take;
     }
@@ -472,10 +689,33 @@ int for_chunks(const step_matrix* list, size_t length, const Visit& visit) {
   return flush();
 }
 
-uint64_t chunk_bytes(const Item* items, int count, bool split) {
-  uint64_t bytes = 0;
-  for (int k = 0; k < count; k++) bytes += planes_of(items[k].m, items[k].n, split).bytes * items[k].count;
-  return bytes;
+// The workspace of one round: its matrices, one behind the other.
+struct Layout {
+  Groups groups;
+  uint32_t counts[kMostGroups];  // matrices of a group
+  uint64_t base[kMostItems];
+  uint64_t bytes;
+};
+
+Layout layout_for(const Item* items, int count, bool split) {
+  Layout l;
+  l.groups.count = 0;
+  l.bytes = 0;
+  uint32_t number = 0;
+  for (int k = 0; k < count; k++) {
+    const Item& item = items[k];
+    l.base[k] = l.bytes;
+    const int g = l.groups.count - 1;
+    if (g >= 0 && l.groups.at[g].m == item.m && l.groups.at[g].n == item.n) {
+      l.counts[g] += static_cast<uint32_t>(item.count);
+    } else {
+      l.groups.at[l.groups.count] = {l.bytes, item.m, item.n, 0, 0, number};
+      l.counts[l.groups.count++] = static_cast<uint32_t>(item.count);
+    }
+    number += static_cast<uint32_t>(item.count);
+    l.bytes += planes_of(item.m, item.n, split).bytes * item.count;
+  }
+  return l;
 }
 
 int check_list(const step_matrix* list, size_t length, int dtype, int out_dtype, bool muon) {
@@ -490,29 +730,82 @@ int check_list(const step_matrix* list, size_t length, int dtype, int out_dtype,
   return STEP_OK;
 }
 
-// By type: the update's T picks the kernels that read it, the result's the one that writes it.
 template <typename Go> void by_type(int dtype, const Go& go) {
   if (dtype == STEP_F32) go(F32());
   else if (dtype == STEP_BF16) go(BF16());
   else go(F16());
 }
 
-template <int TM, int TN, int WM, int WN, Kind KIND, bool SPLIT>
-void launch_product(Groups groups, const uint32_t* counts, char* ws, int from, float a, float b, float c, hipStream_t stream) {
-  uint32_t tiles = 0;
+// What a workgroup of a tile size takes: microseconds per stage of its depth and for what comes behind, where
+// `per_cu` workgroups share a compute unit.
+struct Cost {
+  double stage, end;
+  uint32_t per_cu;
+};
+constexpr uint32_t kUnits = 256;  // compute units
+
+// The tiles of side `side` of a product of every group, and about how long the launch takes.
+template <Kind KIND> double cut(Groups& groups, const uint32_t* counts, uint32_t side, const Cost& cost, uint32_t* tiles) {
+  double work = 0, longest = 0;
+  *tiles = 0;
   for (int k = 0; k < groups.count; k++) {
     Group& g = groups.at[k];
-    const uint32_t down = (g.m + TM - 1) / TM, across = (g.n + TN - 1) / TN;
-    g.tiles = KIND == APPLY ? down * across : down * (down + 1) / 2;
-    g.first_tile = tiles;
-    tiles += g.tiles * counts[k];
+    const uint32_t down = (g.m + side - 1) / side, across = (g.n + side - 1) / side;
+    g.tiles = KIND == APPLY || KIND == LAST ? down * across : down * (down + 1) / 2;
+    g.first_tile = *tiles;
+    *tiles += g.tiles * counts[k];
+    const double one = (KIND == GRAM ? g.n : g.m) / 64 * cost.stage + cost.end;
+    work += one * g.tiles * counts[k];
+    longest = std::max(longest, one);
   }
-  hipLaunchKernelGGL((product_kernel<TM, TN, WM, WN, KIND, SPLIT>), dim3(tiles), dim3(WM * WN * 64), 0, stream, groups, ws, from, a, b, c);
+  const uint32_t at_once = kUnits * cost.per_cu;
+  if (groups.count > 1) return std::max(longest / cost.per_cu, work / at_once);  // unlike tiles fill each other's gaps
+  // alike ones go round by round; a workgroup that has a unit to itself is faster
+  const uint32_t left = *tiles % at_once;
+  return longest * (*tiles / at_once + (left == 0 ? 0 : left <= kUnits ? 1.0 / cost.per_cu : 1.0));
 }
 
-template <Kind KIND, bool SPLIT>
-void product(const Groups& groups, const uint32_t* counts, char* ws, int from, const float* coefficients, hipStream_t stream) {
-  launch_product<128, 128, 2, 2, KIND, SPLIT>(groups, counts, ws, from, coefficients[0], coefficients[1], coefficients[2], stream);
+template <int SIDE, int WM, int WN, int KS, int STAGES, Kind KIND, bool SPLIT, typename Extra>
+void launch_product(const Groups& groups, uint32_t tiles, const Extra& targets, char* ws, int from, int low_in, int low_out,
+                    const float* coefficients, hipStream_t stream) {
+  hipLaunchKernelGGL((product_kernel<SIDE, WM, WN, KS, STAGES, KIND, SPLIT>), dim3(tiles), dim3(KS * WM * WN * 64), 0, stream,
+                     groups, targets, ws, from, low_in, low_out, coefficients[0], coefficients[1], coefficients[2]);
+}
+
+// The tile size by what the launch would take with each. Large tiles read less per product but leave compute units idle
+// where there are few; the costs are those measured for one 1024 x 4096, 16 of 1024 x 1024, 4096 x 4096, 4096 x 16384 and
+// 8192 x 8192. Triangles: 4096 x 16384 half has 136 tiles of 256 (365 us), 253 of 192 (290 us), 528 of 128 (382 us); 1024 x
+// 4096 has 36 of 128 (41 us) and 136 of 64 (15 us).
+template <Kind KIND, bool SPLIT, typename Extra>
+void product(const Layout& l, const Extra& targets, char* ws, int from, int low_in, int low_out, const float* coefficients,
+             hipStream_t stream) {
+  constexpr bool SQUARES = KIND == APPLY || KIND == LAST;
+  Groups groups = l.groups;
+  uint32_t tiles;
+  auto go = [&](auto kernel, uint32_t side) {
+    cut<KIND>(groups, l.counts, side, Cost{0, 0, 1}, &tiles);
+    kernel(groups, tiles);
+  };
+#define STEP_PRODUCT(...)                                                                                            \
+  [&](const Groups& g, uint32_t t) {                                                                                 \
+    launch_product<__VA_ARGS__, KIND, SPLIT>(g, t, targets, ws, from, low_in, low_out, coefficients, stream);        \
+  }
+  if constexpr (SPLIT) {
+    const double large = cut<KIND>(groups, l.counts, 128, Cost{1.1, KIND == LAST ? 18. : KIND == APPLY ? 24. : 10., 1}, &tiles);
+    const double small = cut<KIND>(groups, l.counts, 64, Cost{0.47, SQUARES ? 5.8 : 3.3, 1}, &tiles);
+    if (large < small) go(STEP_PRODUCT(128, 2, 4, 1, 2), 128);
+    else go(STEP_PRODUCT(64, 2, 2, 2, 2), 64);
+  } else {
+    const double t256 = cut<KIND>(groups, l.counts, 256, Cost{1.42, KIND == LAST ? 36. : KIND == APPLY ? 70. : 10., 1}, &tiles);
+    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, l.counts, 192, Cost{1.0, 7., 1}, &tiles);
+    const double t128 = cut<KIND>(groups, l.counts, 128, Cost{1.0, KIND == LAST ? 16. : KIND == APPLY ? 20. : 5., 2}, &tiles);
+    const double t64 = cut<KIND>(groups, l.counts, 64, Cost{0.17, SQUARES ? 4.3 : 2.7, 1}, &tiles);
+    if (t64 <= std::min(std::min(t256, t192), t128)) go(STEP_PRODUCT(64, 2, 2, 2, 4), 64);
+    else if (t128 <= std::min(t256, t192)) go(STEP_PRODUCT(128, 2, 2, 1, 2), 128);
+    else if (t256 <= t192) go(STEP_PRODUCT(256, 2, 4, 1, 2), 256);
+    else if constexpr (!SQUARES) go(STEP_PRODUCT(192, 2, 4, 1, 3), 192);
+  }
+#undef STEP_PRODUCT
 }
 
 struct Rule {
@@ -523,78 +816,58 @@ struct Rule {
 };
 
 template <bool SPLIT>
-int run_chunk(const step_matrix* list, const Item* items, int count, int dtype, int out_dtype, const Rule& rule, char* ws,
+int run_round(const step_matrix* list, const Item* items, int count, int dtype, int out_dtype, const Rule& rule, char* ws,
               hipStream_t stream) {
-  Segments segments;
-  Groups groups;
-  uint32_t counts[kMostSegments];
-  segments.count = count;
-  groups.count = 0;
-  uint64_t at = 0;
+  const Layout l = layout_for(items, count, SPLIT);
+  Segments by_piece, by_tile;
+  Targets targets;
+  by_piece.count = by_tile.count = targets.count = count;
+  targets.type = out_dtype;
+  targets.muon = rule.muon;
+  targets.keep = rule.keep;
+  uint32_t pieces = 0, tiles = 0, number = 0;
   for (int k = 0; k < count; k++) {
     const Item& item = items[k];
     const step_matrix& x = list[item.matrix];
     const uint64_t size = static_cast<uint64_t>(x.rows) * x.cols, skip = item.first * size;
-    Segment& s = segments.at[k];
-    s.grad = static_cast<const char*>(x.grad) + skip * dtype_size(dtype);
-    s.momentum = x.momentum ? x.momentum + skip : nullptr;
-    s.out = static_cast<char*>(x.out) + skip * dtype_size(out_dtype);
-    s.base = at;
-    s.rows = static_cast<uint32_t>(x.rows);
-    s.cols = static_cast<uint32_t>(x.cols);
-    s.rate = x.rate;
-    s.tall = x.rows > x.cols;
-    if (groups.count && groups.at[groups.count - 1].m == item.m && groups.at[groups.count - 1].n == item.n) {
-      counts[groups.count - 1] += static_cast<uint32_t>(item.count);
-    } else {
-      groups.at[groups.count] = {at, item.m, item.n, 0, 0};
-      counts[groups.count++] = static_cast<uint32_t>(item.count);
-    }
-    at += planes_of(item.m, item.n, SPLIT).bytes * item.count;
-  }
-  uint32_t pieces = 0, tiles = 0;
-  Segments by_piece = segments;
-  for (int k = 0; k < count; k++) {
-    Segment& s = segments.at[k];
-    const uint64_t size = static_cast<uint64_t>(s.rows) * s.cols;
-    Segment& q = by_piece.at[k];
-    q.tiles = static_cast<uint32_t>(std::min<uint64_t>(size / 4096 + 1, kNormBlocks));
-    q.first_tile = pieces;
-    pieces += q.tiles * static_cast<uint32_t>(items[k].count);
-    s.tiles = static_cast<uint32_t>(round_up(s.rows, 64) / 64 * (round_up(s.cols, 64) / 64));
-    s.first_tile = tiles;
-    tiles += s.tiles * static_cast<uint32_t>(items[k].count);
+    const uint32_t rows = static_cast<uint32_t>(x.rows), cols = static_cast<uint32_t>(x.cols), many = static_cast<uint32_t>(item.count);
+    const char* grad = static_cast<const char*>(x.grad) + skip * dtype_size(dtype);
+    float* momentum = rule.momentum.use ? x.momentum + skip : nullptr;
+    const uint32_t of_pieces = pieces_of(size), of_tiles = static_cast<uint32_t>(static_cast<uint64_t>(item.m / 64) * (item.n / 64));
+    by_piece.at[k] = {grad, momentum, l.base[k], rows, cols, pieces, of_pieces};
+    by_tile.at[k] = {grad, momentum, l.base[k], rows, cols, tiles, of_tiles};
+    targets.at[k] = {static_cast<char*>(x.out) + skip * dtype_size(out_dtype), rows, cols, number, x.rate};
+    pieces += of_pieces * many;
+    tiles += of_tiles * many;
+    number += many;
   }
   by_type(dtype, [&](auto type) {
     typedef decltype(type) T;
     hipLaunchKernelGGL((norm_kernel<T>), dim3(pieces), dim3(256), 0, stream, by_piece, rule.momentum, ws, SPLIT ? 1 : 0);
-    hipLaunchKernelGGL((first_kernel<T, SPLIT>), dim3(tiles), dim3(256), 0, stream, segments, rule.momentum, rule.eps, ws);
+    hipLaunchKernelGGL((first_kernel<T, SPLIT>), dim3(tiles), dim3(256), 0, stream, by_tile, rule.momentum, rule.eps, ws);
   });
-  int from = 0;
   for (int step = 0; step < rule.steps; step++) {
     const float* c = rule.coefficients + 3 * step;
-    product<GRAM, SPLIT>(groups, counts, ws, from, c, stream);
-    product<SQUARE, SPLIT>(groups, counts, ws, from, c, stream);
-    product<APPLY, SPLIT>(groups, counts, ws, from, c, stream);
-    from ^= 1;
+    const int from = step % 2, left = rule.steps - 1 - step;
+    product<GRAM, SPLIT>(l, Nothing(), ws, from, 0, 0, c, stream);
+    product<SQUARE, SPLIT>(l, Nothing(), ws, from, 0, 0, c, stream);
+    // the low plane of the last iterate but one is left out (the only one of a single step is there already)
+    if (left) product<APPLY, SPLIT>(l, Nothing(), ws, from, 1, left > 1, c, stream);
+    else product<LAST, SPLIT>(l, targets, ws, from, step == 0, 0, c, stream);
   }
-  by_type(out_dtype, [&](auto type) {
-    typedef decltype(type) T;
-    hipLaunchKernelGGL((last_kernel<T, SPLIT>), dim3(tiles), dim3(256), 0, stream, segments, from, rule.muon, rule.keep, static_cast<const char*>(ws));
-  });
   return launched();
 }
 
 int run(const step_matrix* list, size_t length, int dtype, int out_dtype, int precise, const Rule& rule, void* workspace,
         size_t workspace_bytes, hipStream_t stream) {
-  if (rule.steps < 0 || rule.steps > kMostSteps || (rule.steps && !rule.coefficients)) return STEP_ERR_ARGUMENT;
+  if (rule.steps < 1 || rule.steps > kMostSteps || !rule.coefficients) return STEP_ERR_ARGUMENT;
   const size_t need = step_orthogonalize_workspace(list, length, precise);
   if (need == 0) return STEP_OK;
   if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
-  return for_chunks(list, length, [&](const Item* items, int count) {
-    return precise ? run_chunk<true>(list, items, count, dtype, out_dtype, rule, ws, stream)
-                   : run_chunk<false>(list, items, count, dtype, out_dtype, rule, ws, stream);
+  return for_rounds(list, length, [&](const Item* items, int count) {
+    return precise ? run_round<true>(list, items, count, dtype, out_dtype, rule, ws, stream)
+                   : run_round<false>(list, items, count, dtype, out_dtype, rule, ws, stream);
   });
 }
 
@@ -608,8 +881,8 @@ extern "C" {
 size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int precise) {
   uint64_t most = 0;
   if (length && !list) return 0;
-  for_chunks(list, length, [&](const Item* items, int count) {
-    most = std::max(most, chunk_bytes(items, count, precise != 0));
+  for_rounds(list, length, [&](const Item* items, int count) {
+    most = std::max(most, layout_for(items, count, precise != 0).bytes);
     return static_cast<int>(STEP_OK);
   });
   return most;

@@ -247,15 +247,15 @@ _MOST_STEPS = 64
 
 def _coefficients(coefficients, steps, what):
     """`steps` triples (a, b, c) as a C array; one triple stands for every step."""
-    if not 0 <= steps <= _MOST_STEPS:
-        _refuse("%s: %r steps; 0 to %d are possible", what, steps, _MOST_STEPS)
+    if not 1 <= steps <= _MOST_STEPS:
+        _refuse("%s: %r steps; 1 to %d are possible", what, steps, _MOST_STEPS)
     rows = list(coefficients)
     if len(rows) == 3 and not any(hasattr(r, "__len__") for r in rows):
         rows = [rows] * steps
     if len(rows) != steps or any(len(r) != 3 for r in rows):
         _refuse("%s: coefficients are (a, b, c) or one such triple for each of %d steps", what, steps)
     flat = [float(v) for r in rows for v in r]
-    return (ctypes.c_float * max(len(flat), 1))(*flat)
+    return (ctypes.c_float * len(flat))(*flat)
 
 
 def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=None, precise=None):

@@ -129,8 +129,9 @@ def test_batches():
 
 def test_steps_and_coefficients():
     update = gradient(7, 90, 200)
-    assert distance(mpi.orthogonalize(update, steps=0), exact(update, steps=0)) <= SPLIT
-    assert distance(mpi.orthogonalize(update, steps=1), exact(update, steps=1)) <= SPLIT
+    for steps in (1, 2, 3):
+        assert distance(mpi.orthogonalize(update, steps=steps), exact(update, steps=steps)) <= SPLIT
+        assert distance(mpi.orthogonalize(update, steps=steps, precise=False), exact(update, steps=steps)) <= half(update.shape)
     cubic = (1.5, -0.5, 0.0)
     assert distance(mpi.orthogonalize(update, steps=20, coefficients=cubic), exact(update, 20, cubic)) <= 4 * SPLIT
     schedule = [(3.4, -4.7, 2.0), (2.8, -3.0, 1.2), (1.875, -1.25, 0.375)]
@@ -277,7 +278,7 @@ def test_refusals():
     u = torch.zeros(4, 4).cuda()
     vector, cube = torch.nn.Parameter(torch.zeros(4).cuda()), torch.nn.Parameter(torch.zeros(2, 4, 4).cuda())
     for call in (lambda: mpi.orthogonalize(u[0]), lambda: mpi.orthogonalize(u.long()), lambda: mpi.orthogonalize(u.cpu()),
-                 lambda: mpi.orthogonalize(u, dtype=torch.float64), lambda: mpi.orthogonalize(u, steps=-1),
+                 lambda: mpi.orthogonalize(u, dtype=torch.float64), lambda: mpi.orthogonalize(u, steps=0),
                  lambda: mpi.orthogonalize(u, steps=65), lambda: mpi.orthogonalize(u, coefficients=(1.0, 2.0)),
                  lambda: mpi.orthogonalize(u, steps=3, coefficients=[(1.0, 2.0, 3.0)] * 2),
                  lambda: mpi.Muon([vector]), lambda: mpi.Muon([cube]), lambda: mpi.Muon([torch.nn.Parameter(u.double())]),
