@@ -59,10 +59,10 @@ int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const voi
 
 /* out[v, :] = round(scale * sum of f32(grad[t, :]) over the t with ids[t] = v),
  * for every row v < rows (0 where no token has it). The sum is taken in 32 bits
- * in the order of t, runs of more than step_embedding_window(tokens) tokens in
- * pieces of at most that many whose sums are added in order: the same bits on
- * every call. out is contiguous, of grad's type. */
-size_t step_embedding_window(size_t tokens);
+ * in the order of t, for a row with more than step_embedding_piece(tokens) (64 at
+ * least) tokens in pieces of at most that many whose sums are added in order: the
+ * same bits on every call. out is contiguous, of grad's type. */
+size_t step_embedding_piece(size_t tokens);
 size_t step_embedding_gradient_workspace(size_t tokens, size_t rows, size_t width);
 int step_embedding_gradient(const void* ids, int id_type, size_t tokens, const void* grad, int dtype, size_t rows,
                             size_t width, size_t grad_stride, float scale, void* out, void* workspace,

@@ -17,11 +17,14 @@
 //   * up to kOneGroup tokens one workgroup sorts them in LDS: one launch;
 //   * more tokens take two launches per digit (count, then scatter; the scatter
 //     adds up the counts of all tiles itself instead of a scan in between);
-//   * a run longer than a window (a common token: thousands of rows) is cut at
-//     multiples of the window's length; each window's part is summed by
-//     workgroups of its own into 32 bits and the row's lanes add the parts;
-//   * dW's empty rows are found without clearing a table first: begin[v] is
-//     trusted only if the sorted ids say that a run of v begins there.
+//   * the sorted order is cut into windows of 8 places; the lanes of a window sum
+//     and store the runs that begin in it, in batches of 8 rows in flight;
+//   * a run longer than a piece (a common token: thousands of rows) is cut at
+//     multiples of the piece's length; each part is summed by a workgroup of its
+//     own into 32 bits, and a second launch adds the parts in order;
+//   * the same launch clears dW's empty rows, found without clearing a table
+//     first: begin[v] is trusted only if the sorted ids say that a run of v begins
+//     there.
 #include "step_common.h"
 
 namespace step {
@@ -68,25 +71,34 @@ template <typename T> struct Access {
   // rows of odd widths break 16-byte alignment: element-aligned 16-byte accesses
   typedef typename RawOf<T>::type Raw;
   typedef Raw RawU __attribute__((aligned(sizeof(T))));
-  static constexpr int kCount = Vec<T>::kCount;
+  static constexpr uint32_t kCount = Vec<T>::kCount;
 
-  static __device__ __forceinline__ Vec<T> load(const T* p, uint32_t count) {
+  // The first of the columns of a row's vector v. The last vector of a row whose width is no multiple of a vector's ends
+  // with the row, so that it is loaded as a whole too; it stores only what the one before it does not.
+  static __device__ __forceinline__ uint32_t column(uint32_t v, uint32_t width) {
+    return v * kCount + kCount <= width || width < kCount ? v * kCount : width - kCount;
+  }
+  // `width` < kCount: a row narrower than a vector
+  static __device__ __forceinline__ Vec<T> load(const T* p, uint32_t width) {
     Vec<T> v;
-    if (count >= kCount) {
+    if (width >= kCount) {
       v = __builtin_bit_cast(Vec<T>, static_cast<Raw>(*reinterpret_cast<const RawU*>(p)));
     } else {
       v = __builtin_bit_cast(Vec<T>, Raw{0, 0, 0, 0});
-      for (int k = 0; k < kCount; k++)
-        if (static_cast<uint32_t>(k) < count) v.at[k] = p[k];
+      for (uint32_t k = 0; k < kCount; k++)
+        if (k < width) v.at[k] = p[k];
     }
     return v;
   }
-  static __device__ __forceinline__ void store(T* p, Vec<T> v, uint32_t count) {
-    if (count >= kCount) {
+  // vector `vector` of the row that begins at `row`
+  static __device__ __forceinline__ void store(T* row, Vec<T> v, uint32_t vector, uint32_t width) {
+    T* p = row + column(vector, width);
+    if (vector * kCount + kCount <= width) {
       *reinterpret_cast<RawU*>(p) = __builtin_bit_cast(Raw, v);
     } else {
-      for (int k = 0; k < kCount; k++)
-        if (static_cast<uint32_t>(k) < count) p[k] = v.at[k];
+      const uint32_t skip = vector * kCount - column(vector, width);
+      for (uint32_t k = 0; k < kCount; k++)
+        if (k >= skip && k < width) p[k] = v.at[k];
     }
   }
 };
@@ -99,9 +111,9 @@ __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, con
                               uint32_t rows_per_group) {
   constexpr int N = Vec<T>::kCount;
   const uint32_t slot = threadIdx.x / lanes;
-  const uint32_t column = (blockIdx.y * lanes + threadIdx.x % lanes) * N;
-  if (slot >= rows_per_group || column >= width) return;
-  const uint32_t count = width - column;
+  const uint32_t vector = blockIdx.y * lanes + threadIdx.x % lanes;
+  if (slot >= rows_per_group || vector * N >= width) return;
+  const uint32_t column = Access<T>::column(vector, width);
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * rows_per_group * kLookupRows + slot;
   uint32_t key[kLookupRows];
   Vec<T> v[kLookupRows];
@@ -110,13 +122,13 @@ __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, con
     key[k] = t < tokens ? key_of(ids, id_type, static_cast<uint32_t>(t), rows) : rows;
   }
   for (int k = 0; k < kLookupRows; k++)
-    v[k] = Access<T>::load(weight + (key[k] < rows ? key[k] : 0) * weight_stride + column, key[k] < rows ? count : 0);
+    if (key[k] < rows) v[k] = Access<T>::load(weight + key[k] * weight_stride + column, width);
   for (int k = 0; k < kLookupRows; k++) {
     const uint64_t t = first + k * rows_per_group;
     if (t >= tokens) return;
     for (int e = 0; e < N; e++)
       v[k].at[e] = from_float<T>(key[k] < rows ? scale * to_float(v[k].at[e]) : 0.f);
-    Access<T>::store(out + t * width + column, v[k], count);
+    Access<T>::store(out + t * width, v[k], vector, width);
   }
 }
 
@@ -325,7 +337,7 @@ __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const void* ids,
   if (threadIdx.x == 0) *out_count = all;
 }
 
-// Several workgroups: the counts of a tile's digits, counts[digit * tiles + tile].
+// Several workgroups: the counts of a tile's digits, counts[tile * bins + digit].
 __global__ void __launch_bounds__(kSortThreads) count_kernel(const void* ids, int id_type, const uint32_t* in_keys,
                                                              uint32_t tokens, uint32_t rows, uint32_t tile_length,
                                                              int shift, int bits, uint32_t* counts) {
@@ -341,7 +353,7 @@ __global__ void __launch_bounds__(kSortThreads) count_kernel(const void* ids, in
     atomicAdd(&count[(key >> shift) & (bins - 1)], 1u);
   }
   __syncthreads();
-  if (threadIdx.x < bins) counts[static_cast<uint64_t>(threadIdx.x) * gridDim.x + blockIdx.x] = count[threadIdx.x];
+  if (threadIdx.x < bins) counts[static_cast<uint64_t>(blockIdx.x) * bins + threadIdx.x] = count[threadIdx.x];
 }
 
 // The scatter of a digit's pass. A digit's keys of this tile go behind all smaller digits' keys and those of the same
@@ -357,9 +369,9 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const void* ids, 
   const uint32_t bins = 1u << bits;
   uint32_t in_earlier = 0, in_all = 0;
   if (threadIdx.x < bins) {
-    const uint32_t* row = counts + static_cast<uint64_t>(threadIdx.x) * gridDim.x;
+#pragma unroll 8
     for (uint32_t b = 0; b < gridDim.x; b++) {
-      const uint32_t c = row[b];
+      const uint32_t c = counts[static_cast<uint64_t>(b) * bins + threadIdx.x];
       if (b < blockIdx.x) in_earlier += c;
       in_all += c;
     }
@@ -441,21 +453,32 @@ __global__ void __launch_bounds__(kSortThreads) number_runs_kernel(const uint32_
   group_scan(s, earlier, &number);
   group_scan(s, in_all, &total);
   const uint64_t tile = static_cast<uint64_t>(blockIdx.x) * tile_length;
-  for (uint32_t part = 0; part < tile_length; part += kSortThreads) {
-    const uint64_t i = tile + part + threadIdx.x;
-    const bool begins = begins_run(keys, i, tokens, rows);
+  for (uint32_t part = 0; part < tile_length; part += kTile) {
+    // kTileKeys places of a lane, one behind the other
+    const uint64_t first = tile + part + threadIdx.x * kTileKeys;
+    uint32_t key[kTileKeys + 2], mine = 0;  // and the places before and behind them
+    bool begins[kTileKeys];
+    for (int k = 0; k < kTileKeys + 2; k++) {
+      const uint64_t i = first + k - 1;
+      key[k] = i < tokens ? keys[i] : 0xffffffffu;  // before the first place, i wraps
+    }
+    for (int k = 0; k < kTileKeys; k++) {
+      begins[k] = key[k + 1] < rows && key[k + 1] != key[k];
+      mine += begins[k];
+    }
     uint32_t here;
-    const uint32_t before = group_scan(s, begins ? 1 : 0, &here);
-    if (i < tokens) {
-      const uint32_t key = keys[i];
-      const uint32_t run = number + before + (begins ? 1 : 0) - 1;
-      to.row_of[i] = key < rows ? run : rows;
-      if (begins) {
+    uint32_t run = number + group_scan(s, mine, &here);  // runs that begin before this place
+    for (int k = 0; k < kTileKeys; k++) {
+      const uint64_t i = first + k;
+      if (i >= tokens) break;
+      if (begins[k]) {
         to.begin[run] = static_cast<uint32_t>(i);
-        if (id_type == STEP_I32) static_cast<int32_t*>(out_ids)[run] = static_cast<int32_t>(key);
-        else static_cast<int64_t*>(out_ids)[run] = key;
+        if (id_type == STEP_I32) static_cast<int32_t*>(out_ids)[run] = static_cast<int32_t>(key[k + 1]);
+        else static_cast<int64_t*>(out_ids)[run] = key[k + 1];
+        run++;
       }
-      if (key < rows && (i + 1 == tokens || keys[i + 1] >= rows)) to.begin[total] = static_cast<uint32_t>(i + 1);
+      to.row_of[i] = key[k + 1] < rows ? run - 1 : rows;
+      if (key[k + 1] < rows && key[k + 2] >= rows) to.begin[total] = static_cast<uint32_t>(i + 1);  // the last run's end
     }
     number += here;
   }
@@ -464,96 +487,176 @@ __global__ void __launch_bounds__(kSortThreads) number_runs_kernel(const uint32_
 
 // ---- sums ------------------------------------------------------------------------
 
-// acc += the rows order[b] .. order[e - 1] of `values`, in that order, at one lane's columns.
-template <typename T>
-__device__ __forceinline__ void add_rows(float (&acc)[Vec<T>::kCount], const T* values, uint64_t stride,
-                                         const uint32_t* order, uint32_t b, uint32_t e, uint32_t count) {
-  constexpr int N = Vec<T>::kCount;
-  auto add = [&](auto steps) {
-    constexpr int U = decltype(steps)::value;
-    Vec<T> v[U];
-    for (int k = 0; k < U; k++) v[k] = Access<T>::load(values + order[b + k] * stride, count);
-    for (int k = 0; k < U; k++)
-      for (int n = 0; n < N; n++) acc[n] += to_float(v[k].at[n]);
-    b += U;
-  };
-  while (e - b >= 8) add(std::integral_constant<int, 8>());
-  if (e - b >= 4) add(std::integral_constant<int, 4>());
-  if (e - b >= 2) add(std::integral_constant<int, 2>());
-  if (e - b >= 1) add(std::integral_constant<int, 1>());
+constexpr uint32_t kWindow = 8;     // places of the sorted order whose runs one row of lanes sums
+constexpr uint32_t kNoRow = 0xffffffffu;
+constexpr uint32_t kZeroRows = 64;  // rows of a workgroup that looks for empty ones
+
+struct Sums {
+  uint64_t stride, parts_stride;
+  uint32_t tokens, rows, width;
+  float scale;
+  Sorted by;
+  uint32_t piece, pieces;                   // length of a long run's parts, and how many places of that length there are
+  uint32_t lanes, rows_per_group, chunks;   // RowShape
+  uint32_t piece_groups, window_groups;     // workgroups of the parts and of the windows; the rest clear
+};
+
+template <typename T> __device__ __forceinline__ void add(float (&acc)[Vec<T>::kCount], const Vec<T>& v) {
+  for (int n = 0; n < Vec<T>::kCount; n++) acc[n] += to_float(v.at[n]);
 }
 
-// The parts of long runs: window j holds the places j * window .. of the sorted order. At most two long runs have a
-// part in it, that of its first place (parts[2 j]) and that of its last (parts[2 j + 1]).
 template <typename T>
-__global__ void window_kernel(const T* values, uint64_t stride, uint32_t tokens, uint32_t rows, uint32_t width, Sorted by,
-                              int numbered, uint32_t window, uint32_t lanes, float* parts, uint64_t parts_stride) {
-  constexpr int N = Vec<T>::kCount;
-  const uint32_t column = (blockIdx.y * lanes + threadIdx.x) * N;
-  if (column >= width) return;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * window;
-  const uint32_t last = tokens - first < window ? tokens - 1 : static_cast<uint32_t>(first) + window - 1;
-  for (int side = 0; side < 2; side++) {
-    const uint32_t place = side ? last : static_cast<uint32_t>(first);
-    const uint32_t run = by.row_of[place];
-    if (run >= rows || (side && run == by.row_of[first])) continue;
-    const uint32_t b = by.begin[run], e = numbered ? by.begin[run + 1] : by.end[run];
-    if (e - b <= window) continue;
-    float acc[N] = {};
-    add_rows<T>(acc, values + column, stride, by.order, b > first ? b : static_cast<uint32_t>(first),
-                e <= last ? e : last + 1, width - column);
-    float* to = parts + (static_cast<uint64_t>(blockIdx.x) * 2 + side) * parts_stride + column;
-    for (int n = 0; n < N; n++) to[n] = acc[n];
-  }
+__device__ __forceinline__ void put(T* row, const float (&acc)[Vec<T>::kCount], float scale, uint32_t vector, uint32_t width) {
+  Vec<T> v;
+  for (int n = 0; n < Vec<T>::kCount; n++) v.at[n] = from_float<T>(scale * acc[n]);
+  Access<T>::store(row, v, vector, width);
 }
 
-constexpr int kSumRows = 4;  // rows of a lane slot
-
-template <typename T, bool NUMBERED>
-__global__ void sum_kernel(const T* values, uint64_t stride, uint32_t tokens, uint32_t rows, uint32_t width, float scale,
-                           Sorted by, const int64_t* run_count, uint32_t window, const float* parts,
-                           uint64_t parts_stride, T* out, uint32_t lanes, uint32_t rows_per_group) {
+// The runs that begin in a window and are no longer than a piece. A run's rows are added in the order of the tokens.
+template <typename T>
+__device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* out, uint32_t window, uint32_t vector) {
   constexpr int N = Vec<T>::kCount;
-  const uint32_t slot = threadIdx.x / lanes;
-  const uint32_t column = (blockIdx.y * lanes + threadIdx.x % lanes) * N;
-  if (slot >= rows_per_group || column >= width) return;
-  const uint32_t count = width - column;
-  const uint64_t runs = NUMBERED ? static_cast<uint64_t>(*run_count) : rows;
-  const uint64_t first = static_cast<uint64_t>(blockIdx.x) * rows_per_group * kSumRows + slot;
-  uint32_t b[kSumRows], e[kSumRows];
-  for (int k = 0; k < kSumRows; k++) {
-    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
-    b[k] = r < runs ? by.begin[r] : 0xffffffffu;
-  }
-  for (int k = 0; k < kSumRows; k++) {
-    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
-    e[k] = 0;
-    if (r >= runs) continue;
-    if (NUMBERED) {
-      e[k] = by.begin[r + 1];
-    } else {
-      // begin[r] holds anything if no token has row r: a run of r begins there only if the sorted ids say so
-      const bool begins = b[k] < tokens && by.row_of[b[k]] == r && (b[k] == 0 || by.row_of[b[k] - 1] != r);
-      if (begins) e[k] = by.end[r];
-      else b[k] = 0;
+  const uint32_t column = Access<T>::column(vector, q.width);
+  const uint64_t w0 = static_cast<uint64_t>(window) * kWindow, w1 = w0 + kWindow;
+  auto row_at = [&](uint64_t i) { return i < q.tokens ? q.by.row_of[i] : kNoRow; };
+  float acc[N];
+  uint32_t before = w0 ? q.by.row_of[w0 - 1] : kNoRow, open = kNoRow;  // open: the row being summed
+  for (uint64_t i = w0;; i += 8) {
+    uint32_t row[8], ahead[8], order[8];
+    for (int k = 0; k < 8; k++) {
+      row[k] = row_at(i + k);
+      ahead[k] = row_at(i + k + q.piece);
+      order[k] = i + k < q.tokens ? q.by.order[i + k] : 0;
     }
-  }
-  for (int k = 0; k < kSumRows; k++) {
-    const uint64_t r = first + static_cast<uint64_t>(k) * rows_per_group;
-    if (r >= runs) return;
-    float acc[N] = {};
-    if (e[k] - b[k] <= window) {
-      add_rows<T>(acc, values + column, stride, by.order, b[k], e[k], count);
-    } else {
-      for (uint32_t j = b[k] / window; j <= (e[k] - 1) / window; j++) {
-        const uint64_t part = static_cast<uint64_t>(j) * 2 + (b[k] > j * window ? 1 : 0);
-        for (int n = 0; n < N; n++) acc[n] += parts[part * parts_stride + column + n];
+    // what each place does: nothing, begin a run, go on with it
+    bool take[8], begin[8], stop = false;
+    for (int k = 0; k < 8; k++) {
+      take[k] = begin[k] = false;
+      if (stop) continue;
+      if (row[k] != before) {
+        before = row[k];
+        // the end: of the window, of the rows (dropped ids and the places behind the last have larger numbers), or a
+        // long run, which lasts beyond the window
+        if (i + k >= w1 || row[k] >= q.rows || ahead[k] == row[k]) stop = true;
+        else take[k] = begin[k] = true;
+      } else {
+        take[k] = open != kNoRow || (k && take[k - 1]);
+        if (!take[k] && i + k >= w1) stop = true;                 // a run that began before the window and outlasts it
       }
     }
-    Vec<T> v;
-    for (int n = 0; n < N; n++) v.at[n] = from_float<T>(scale * acc[n]);
-    Access<T>::store(out + r * width + column, v, count);
+    Vec<T> v[8];
+    for (int k = 0; k < 8; k++)
+      if (take[k]) v[k] = Access<T>::load(values + order[k] * q.stride + column, q.width);
+    for (int k = 0; k < 8; k++) {
+      if (!take[k]) continue;
+      if (begin[k]) {
+        if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+        open = row[k];
+        for (int n = 0; n < N; n++) acc[n] = 0.f;
+      }
+      add<T>(acc, v[k]);
+    }
+    if (stop || (open == kNoRow && i + 8 >= w1)) break;
   }
+  if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+}
+
+// A long run's part: piece j holds the places j * piece .. of the sorted order. At most two long runs have a part in it,
+// that of its first place (parts[2 j]) and that of its last (parts[2 j + 1]).
+template <typename T, bool NUMBERED>
+__device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float* parts, uint32_t piece, uint32_t vector) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t column = Access<T>::column(vector, q.width);
+  const uint64_t first = static_cast<uint64_t>(piece) * q.piece;
+  const uint32_t last = q.tokens - first < q.piece ? q.tokens - 1 : static_cast<uint32_t>(first) + q.piece - 1;
+  for (int side = 0; side < 2; side++) {
+    const uint32_t place = side ? last : static_cast<uint32_t>(first);
+    const uint32_t run = q.by.row_of[place];
+    if (run >= q.rows || (side && run == q.by.row_of[first])) continue;
+    const uint32_t b = q.by.begin[run], e = NUMBERED ? q.by.begin[run + 1] : q.by.end[run];
+    if (e - b <= q.piece) continue;
+    uint32_t i = b > first ? b : static_cast<uint32_t>(first);
+    const uint32_t end = e <= last ? e : last + 1;
+    float acc[N] = {};
+    for (; i + 8 <= end; i += 8) {
+      Vec<T> v[8];
+      for (int k = 0; k < 8; k++) v[k] = Access<T>::load(values + q.by.order[i + k] * q.stride + column, q.width);
+      for (int k = 0; k < 8; k++) add<T>(acc, v[k]);
+    }
+    for (; i < end; i++) add<T>(acc, Access<T>::load(values + q.by.order[i] * q.stride + column, q.width));
+    float* to = parts + (static_cast<uint64_t>(piece) * 2 + side) * q.parts_stride + column;
+    const uint32_t skip = vector * N - column;   // what the vector before stores
+    for (int n = 0; n < N; n++)
+      if (static_cast<uint32_t>(n) >= skip) to[n] = acc[n];
+  }
+}
+
+template <typename T, bool NUMBERED>
+__global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float* parts, T* out) {
+  __shared__ uint32_t empty[kZeroRows];
+  if (blockIdx.x < q.piece_groups + q.window_groups) {
+    const bool pieces = blockIdx.x < q.piece_groups;
+    const uint32_t group = pieces ? blockIdx.x : blockIdx.x - q.piece_groups;
+    const uint32_t slot = threadIdx.x / q.lanes, vector = group % q.chunks * q.lanes + threadIdx.x % q.lanes;
+    if (slot >= q.rows_per_group || vector * Vec<T>::kCount >= q.width) return;
+    const uint32_t number = group / q.chunks * q.rows_per_group + slot;
+    if (pieces) {
+      if (number < q.pieces) sum_piece<T, NUMBERED>(q, values, parts, number, vector);
+    } else if (static_cast<uint64_t>(number) * kWindow < q.tokens) {
+      sum_window<T>(q, values, out, number, vector);
+    }
+    return;
+  }
+  // rows that no token has; not of numbered runs, which have none
+  const uint64_t first = static_cast<uint64_t>(blockIdx.x - q.piece_groups - q.window_groups) * kZeroRows;
+  for (uint32_t k = threadIdx.x; k < kZeroRows; k += 256) {
+    const uint64_t r = first + k;
+    // begin[r] holds anything if no token has row r: a run of r begins there only if the sorted ids say so
+    bool begins = false;
+    if (r < q.rows) {
+      const uint32_t b = q.by.begin[r];
+      begins = b < q.tokens && q.by.row_of[b] == r && (b == 0 || q.by.row_of[b - 1] != r);
+    }
+    empty[k] = r < q.rows && !begins;
+  }
+  __syncthreads();
+  const uint32_t vectors = (q.width + Vec<T>::kCount - 1) / Vec<T>::kCount;
+  const float zero[Vec<T>::kCount] = {};
+  // whole waves go along a row
+  const uint32_t per_row = vectors < 64 ? vectors : (vectors + 63) / 64 * 64;
+  for (uint32_t at = threadIdx.x; at < kZeroRows * static_cast<uint64_t>(per_row); at += 256) {
+    const uint32_t k = at / per_row, vector = at % per_row;
+    if (vector < vectors && empty[k]) put<T>(out + (first + k) * q.width, zero, 1.f, vector, q.width);
+  }
+}
+
+// Long runs: the parts of the run that begins in piece j, in order.
+template <typename T, bool NUMBERED>
+__global__ void __launch_bounds__(256) join_kernel(Sums q, const float* parts, T* out) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t slot = threadIdx.x / q.lanes, vector = blockIdx.x % q.chunks * q.lanes + threadIdx.x % q.lanes;
+  const uint32_t piece = blockIdx.x / q.chunks * q.rows_per_group + slot;
+  if (slot >= q.rows_per_group || vector * N >= q.width || piece >= q.pieces) return;
+  const uint32_t column = Access<T>::column(vector, q.width);
+  const uint64_t first = static_cast<uint64_t>(piece) * q.piece;
+  const uint32_t run = q.by.row_of[q.tokens - first < q.piece ? q.tokens - 1 : static_cast<uint32_t>(first) + q.piece - 1];
+  if (run >= q.rows) return;
+  const uint32_t b = q.by.begin[run], e = NUMBERED ? q.by.begin[run + 1] : q.by.end[run];
+  if (e - b <= q.piece || b < first) return;
+  float acc[N] = {};
+  auto part = [&](uint32_t j) { return parts + (static_cast<uint64_t>(j) * 2 + (b > static_cast<uint64_t>(j) * q.piece ? 1 : 0)) * q.parts_stride + column; };
+  const uint32_t end = (e - 1) / q.piece + 1;
+  uint32_t j = piece;
+  for (; j + 8 <= end; j += 8) {
+    float v[8][N];
+    for (int k = 0; k < 8; k++)
+      for (int n = 0; n < N; n++) v[k][n] = part(j + k)[n];
+    for (int k = 0; k < 8; k++)
+      for (int n = 0; n < N; n++) acc[n] += v[k][n];
+  }
+  for (; j < end; j++)
+    for (int n = 0; n < N; n++) acc[n] += part(j)[n];
+  put<T>(out + static_cast<uint64_t>(run) * q.width, acc, q.scale, vector, q.width);
 }
 
 // ---- host side --------------------------------------------------------------------
@@ -561,14 +664,14 @@ __global__ void sum_kernel(const T* values, uint64_t stride, uint32_t tokens, ui
 // The pieces of a workspace, each on a 256-byte boundary.
 struct Layout {
   size_t keys[2], order[2], counts, row_of, begin, end, parts, bytes;
-  uint32_t tile_length, tiles, window, windows;
+  uint32_t tile_length, tiles, piece, pieces;
   size_t parts_stride;
 };
 
-uint32_t window_for(size_t tokens) {
-  // a long run costs tokens / windows row additions in a row, then one for each window: balanced at the square root
+// A long run costs the additions of a part in a row, then one for each part: the longest are balanced at the square root.
+uint32_t piece_for(size_t tokens) {
   uint32_t w = 64;
-  while (static_cast<size_t>(w) * w < tokens) w *= 2;
+  while (static_cast<size_t>(w) * w * 4 < tokens) w *= 2;
   return w;
 }
 
@@ -580,8 +683,8 @@ Layout layout_for(size_t tokens, size_t rows, size_t width, bool numbered) {
     at += round_up(bytes, 256);
     return here;
   };
-  l.window = window_for(tokens);
-  l.windows = static_cast<uint32_t>((tokens + l.window - 1) / l.window);
+  l.piece = piece_for(tokens);
+  l.pieces = tokens > l.piece ? static_cast<uint32_t>((tokens + l.piece - 1) / l.piece) : 0;  // else no run is longer
   l.tile_length = kTile;
   if (tokens > static_cast<size_t>(kTile) * kMostTiles)
     l.tile_length = static_cast<uint32_t>(round_up((tokens + kMostTiles - 1) / kMostTiles, kTile));
@@ -597,7 +700,7 @@ Layout layout_for(size_t tokens, size_t rows, size_t width, bool numbered) {
   l.begin = take(runs * 4);
   l.end = numbered ? l.begin : take(runs * 4);
   l.parts_stride = round_up(width, 64);
-  l.parts = take(tokens > l.window ? static_cast<size_t>(l.windows) * 2 * l.parts_stride * 4 : 0);
+  l.parts = take(static_cast<size_t>(l.pieces) * 2 * l.parts_stride * 4);
   l.bytes = at ? at : 256;
   return l;
 }
@@ -646,24 +749,19 @@ Sorted sort_tokens(const Layout& l, char* ws, const void* ids, int id_type, uint
 
 template <typename T, bool NUMBERED>
 void sum_rows(const Layout& l, char* ws, const Sorted& by, const void* values, uint64_t stride, uint32_t tokens,
-              uint32_t rows, uint32_t width, float scale, const int64_t* run_count, void* out, hipStream_t stream) {
-  const size_t vectors = (width + Vec<T>::kCount - 1) / Vec<T>::kCount;
+              uint32_t rows, uint32_t width, float scale, void* out, hipStream_t stream) {
+  const RowShape s = row_shape((width + Vec<T>::kCount - 1) / Vec<T>::kCount);
   float* parts = reinterpret_cast<float*>(ws + l.parts);
-  if (tokens > l.window) {
-    RowShape w = row_shape(vectors);
-    // one row of lanes per workgroup, whole waves of it
-    const uint32_t threads = w.lanes < 64 ? 64 : w.lanes;
-    hipLaunchKernelGGL((window_kernel<T>), dim3(l.windows, w.chunks), dim3(threads), 0, stream,
-                       static_cast<const T*>(values), stride, tokens, rows, width, by, NUMBERED ? 1 : 0, l.window, threads,
-                       parts, static_cast<uint64_t>(l.parts_stride));
-  }
-  const RowShape s = row_shape(vectors);
-  const uint64_t most = NUMBERED ? (tokens < rows ? tokens : rows) : rows;
-  const uint64_t per_group = static_cast<uint64_t>(s.rows_per_group) * kSumRows;
-  hipLaunchKernelGGL((sum_kernel<T, NUMBERED>), dim3(static_cast<uint32_t>((most + per_group - 1) / per_group), s.chunks),
-                     dim3(256), 0, stream, static_cast<const T*>(values), stride, tokens, rows, width, scale, by, run_count,
-                     l.window, static_cast<const float*>(parts), static_cast<uint64_t>(l.parts_stride),
-                     static_cast<T*>(out), s.lanes, s.rows_per_group);
+  auto groups = [&](uint64_t number) { return static_cast<uint32_t>((number + s.rows_per_group - 1) / s.rows_per_group * s.chunks); };
+  Sums q = {stride, l.parts_stride, tokens, rows, width, scale, by, l.piece, l.pieces, s.lanes, s.rows_per_group, s.chunks, 0, 0};
+  q.piece_groups = groups(l.pieces);
+  q.window_groups = groups((tokens + kWindow - 1) / kWindow);
+  const uint32_t clearing = NUMBERED ? 0 : (rows + kZeroRows - 1) / kZeroRows;
+  hipLaunchKernelGGL((sum_kernel<T, NUMBERED>), dim3(q.piece_groups + q.window_groups + clearing), dim3(256), 0, stream, q,
+                     static_cast<const T*>(values), parts, static_cast<T*>(out));
+  if (l.pieces)
+    hipLaunchKernelGGL((join_kernel<T, NUMBERED>), dim3(q.piece_groups), dim3(256), 0, stream, q,
+                       static_cast<const float*>(parts), static_cast<T*>(out));
 }
 
 __global__ void zero_kernel(uint32_t* to, uint64_t words, uint16_t* tail, int has_tail) {
@@ -738,7 +836,7 @@ int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const voi
   return launched();
 }
 
-size_t step_embedding_window(size_t tokens) { return window_for(tokens); }
+size_t step_embedding_piece(size_t tokens) { return piece_for(tokens); }
 
 size_t step_embedding_gradient_workspace(size_t tokens, size_t rows, size_t width) {
   if (tokens > kMostSize || rows > kMostSize || width > kMostSize) return 0;
@@ -766,9 +864,9 @@ int step_embedding_gradient(const void* ids, int id_type, size_t tokens, const v
   char* ws = static_cast<char*>(workspace);
   const uint32_t t = static_cast<uint32_t>(tokens), v = static_cast<uint32_t>(rows), w = static_cast<uint32_t>(width);
   const Sorted by = sort_tokens(l, ws, ids, id_type, t, v, false, nullptr, nullptr, stream);
-  if (dtype == STEP_F32) sum_rows<F32, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
-  else if (dtype == STEP_BF16) sum_rows<BF16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
-  else sum_rows<F16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, nullptr, out, stream);
+  if (dtype == STEP_F32) sum_rows<F32, false>(l, ws, by, grad, grad_stride, t, v, w, scale, out, stream);
+  else if (dtype == STEP_BF16) sum_rows<BF16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, out, stream);
+  else sum_rows<F16, false>(l, ws, by, grad, grad_stride, t, v, w, scale, out, stream);
   return launched();
 }
 
@@ -796,9 +894,9 @@ int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* val
   const uint32_t t = static_cast<uint32_t>(tokens), v = static_cast<uint32_t>(rows), w = static_cast<uint32_t>(width);
   const Sorted by = sort_tokens(l, ws, ids, id_type, t, v, true, out_ids, out_count, stream);
   if (width == 0) return launched();
-  if (dtype == STEP_F32) sum_rows<F32, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
-  else if (dtype == STEP_BF16) sum_rows<BF16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
-  else sum_rows<F16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_count, out_values, stream);
+  if (dtype == STEP_F32) sum_rows<F32, true>(l, ws, by, values, values_stride, t, v, w, scale, out_values, stream);
+  else if (dtype == STEP_BF16) sum_rows<BF16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_values, stream);
+  else sum_rows<F16, true>(l, ws, by, values, values_stride, t, v, w, scale, out_values, stream);
   return launched();
 }
 

@@ -17,7 +17,7 @@ LIB_PATH = os.path.join(_PKG_ROOT, "lib", "libstep_hip.so")
 # Every symbol include/step_abi.h declares.
 EXPORTS = (
     "step_abi_version", "step_status_string", "step_last_hip_error",
-    "step_embedding_lookup", "step_embedding_window", "step_embedding_gradient_workspace", "step_embedding_gradient",
+    "step_embedding_lookup", "step_embedding_piece", "step_embedding_gradient_workspace", "step_embedding_gradient",
     "step_sum_slices_workspace", "step_sum_slices",
     "step_orthogonalize_workspace", "step_orthogonalize", "step_muon",
 )
@@ -58,7 +58,7 @@ def lib():
             "step_status_string": (ctypes.c_char_p, [ci]),
             "step_last_hip_error": (ci, []),
             "step_embedding_lookup": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp]),
-            "step_embedding_window": (sz, [sz]),
+            "step_embedding_piece": (sz, [sz]),
             "step_embedding_gradient_workspace": (sz, [sz, sz, sz]),
             "step_embedding_gradient": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp, sz, vp]),
             "step_sum_slices_workspace": (sz, [sz, sz, sz]),

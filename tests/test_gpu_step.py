@@ -134,7 +134,7 @@ def test_gradient(shape, dtype):
 
 
 def test_gradient_adds_in_the_order_of_the_tokens():
-    """Up to a window's length (64 tokens at least) a row's sum is the left fold over its tokens, bit for bit."""
+    """Up to a piece's length (64 tokens at least) a row's sum is the left fold over its tokens, bit for bit."""
     tokens, rows, width = 3000, 128, 37
     grad, ids = values(7, tokens, width), make_ids(8, tokens, rows, "any", torch.int64)
     assert int(torch.bincount(ids).max()) <= 64

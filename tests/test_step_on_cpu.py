@@ -31,10 +31,10 @@ def test_binding_covers_the_header():
         assert lib.step_status_string(status)
 
 
-def test_window_is_the_square_root_and_at_least_64():
+def test_pieces_are_half_the_square_root_and_at_least_64():
     lib = step_abi.lib()
-    for tokens, window in ((0, 64), (1, 64), (4096, 64), (4097, 128), (16384, 128), (1 << 20, 1024)):
-        assert lib.step_embedding_window(tokens) == window
+    for tokens, piece in ((0, 64), (1, 64), (16384, 64), (16385, 128), (65536, 128), (1 << 20, 512)):
+        assert lib.step_embedding_piece(tokens) == piece
 
 
 def test_workspace_of_sizes_that_do_not_fit_is_zero():
@@ -136,5 +136,5 @@ def test_embedding_assembly():
     text = _assembly(EMBEDDING)
     found = stale_selects(text)
     assert not found, "scalar selects on a stale condition code: %r" % (found[:5],)
-    kernels = kernels_in_scratch(text, ("lookup_kernel", "sort_one_kernel", "scatter_kernel", "window_kernel", "sum_kernel"))
+    kernels = kernels_in_scratch(text, ("lookup_kernel", "sort_one_kernel", "scatter_kernel", "sum_kernel", "join_kernel"))
     assert kernels["seen"] >= 17 and not kernels["scratch"], kernels
