@@ -41,7 +41,7 @@ def _check_tensor(t, name, types, what):
 
 
 def _same_device(what, a, b):
-    if a.device != b.device:
+    if a.get_device() != b.get_device():
         _refuse("%s: tensors on %s and %s", what, a.device, b.device)
 
 
@@ -52,38 +52,36 @@ def _rows_of(t):
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
-class _on:
-    """The tensors' device as the current one (entered only if it is not), and its current stream."""
-
-    def __init__(self, device):
-        self._index = device.index
-        self._guard = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self._index:
-            self._guard = torch.cuda.device(self._index)
-            self._guard.__enter__()
-        return torch.cuda.current_stream(self._index).cuda_stream
-
-    def __exit__(self, *exc):
-        if self._guard is not None:
-            self._guard.__exit__(*exc)
-        return False
+# The current stream and device as plain numbers: these calls are a large part of a small operator's time, and in a
+# backward pass, which runs on a thread of autograd's own, every Python object that is touched comes from another core.
+_stream_of = torch._C._cuda_getCurrentRawStream
+_current_device = torch._C._cuda_getDevice
+_empty = torch.empty
 
 
-def _workspace(size, device):
-    return torch.empty(size, dtype=torch.uint8, device=device)
+def _on_device(fn, tensor, *args):
+    """fn(*args) with the tensor's device as the current one."""
+    with torch.cuda.device(tensor.device):
+        return fn(*args)
 
 
 def _lookup(ids, weight, scale):
-    ids = ids.contiguous()
-    weight, stride = _rows_of(weight)
+    index = weight.get_device()
+    if index != _current_device():
+        return _on_device(_lookup, weight, ids, weight, scale)
     rows, width = weight.shape
-    out = torch.empty(ids.shape + (width,), dtype=weight.dtype, device=weight.device)
-    with _on(weight.device) as stream:
-        step_abi.check(step_abi.lib().step_embedding_lookup(
-            ids.data_ptr(), _IDS[ids.dtype], ids.numel(), weight.data_ptr(), _FLOATS[weight.dtype], rows, width, stride,
-            scale, out.data_ptr(), stream), "embedding")
+    stride = width
+    if not weight.is_contiguous():
+        weight, stride = _rows_of(weight)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    dtype = weight.dtype
+    out = _empty((*ids.shape, width), dtype=dtype, device=weight.device)
+    status = (step_abi._lib or step_abi.lib()).step_embedding_lookup(
+        ids.data_ptr(), _IDS[ids.dtype], ids.numel(), weight.data_ptr(), _FLOATS[dtype], rows, width, stride, scale,
+        out.data_ptr(), _stream_of(index))
+    if status:
+        step_abi.check(status, "embedding")
     return out
 
 
@@ -115,18 +113,25 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
 
 
 def _gradient(grad, ids, rows, scale):
-    ids = ids.contiguous()
-    width = grad.shape[-1]
-    grad, stride = _rows_of(grad.reshape(-1, width) if grad.numel() else grad.new_empty(ids.numel(), width))
-    tokens = grad.shape[0]
-    out = torch.empty(rows, width, dtype=grad.dtype, device=grad.device)
-    L = step_abi.lib()
-    with _on(grad.device) as stream:
-        size = L.step_embedding_gradient_workspace(tokens, rows, width)
-        ws = _workspace(size, grad.device)
-        step_abi.check(L.step_embedding_gradient(
-            ids.data_ptr(), _IDS[ids.dtype], tokens, grad.data_ptr(), _FLOATS[grad.dtype], rows, width, stride, scale,
-            out.data_ptr(), ws.data_ptr(), size, stream), "embedding_gradient")
+    index = grad.get_device()
+    if index != _current_device():
+        return _on_device(_gradient, grad, grad, ids, rows, scale)
+    if not ids.is_contiguous():
+        ids = ids.contiguous()
+    tokens, width = ids.numel(), grad.shape[-1]
+    stride = width
+    if not grad.is_contiguous():
+        grad, stride = _rows_of(grad.reshape(tokens, width))
+    dtype, device = grad.dtype, grad.device
+    out = _empty((rows, width), dtype=dtype, device=device)
+    L = step_abi._lib or step_abi.lib()
+    size = L.step_embedding_gradient_workspace(tokens, rows, width)
+    ws = _empty(size, dtype=torch.uint8, device=device)
+    status = L.step_embedding_gradient(
+        ids.data_ptr(), _IDS[ids.dtype], tokens, grad.data_ptr(), _FLOATS[dtype], rows, width, stride, scale,
+        out.data_ptr(), ws.data_ptr(), size, _stream_of(index))
+    if status:
+        step_abi.check(status, "embedding_gradient")
     return out
 
 
@@ -167,48 +172,65 @@ def sum_slices(slices):
 
 
 def _sum_slices(values, indices, rows, scale):
-    shape = values.shape[1:]
-    tokens, width = indices.shape[0], 1
-    for d in shape:
-        width *= d
+    index = values.get_device()
+    if index != _current_device():
+        return _on_device(_sum_slices, values, values, indices, rows, scale)
+    shape, dtype, device = tuple(values.shape[1:]), values.dtype, values.device
+    tokens, width = indices.shape[0], math.prod(shape)
     flat, stride = _rows_of(values.reshape(tokens, width))
     indices = indices.contiguous()
     most = min(tokens, rows)
-    out_ids = torch.empty(most, dtype=indices.dtype, device=values.device)
-    out = torch.empty(most, width, dtype=values.dtype, device=values.device)
-    count = torch.empty(1, dtype=torch.int64, device=values.device)
-    L = step_abi.lib()
-    with _on(values.device) as stream:
-        size = L.step_sum_slices_workspace(tokens, rows, width)
-        ws = _workspace(size, values.device)
-        step_abi.check(L.step_sum_slices(
-            indices.data_ptr(), _IDS[indices.dtype], tokens, flat.data_ptr(), _FLOATS[values.dtype], rows, width, stride,
-            scale, out_ids.data_ptr(), out.data_ptr(), count.data_ptr(), ws.data_ptr(), size, stream), "sum_slices")
-    n = int(count.item())
-    return out_ids[:n], out[:n].reshape((n,) + tuple(shape))
+    out_ids = _empty(most, dtype=indices.dtype, device=device)
+    out = _empty((most, width), dtype=dtype, device=device)
+    count = _empty(1, dtype=torch.int64, device=device)
+    L = step_abi._lib or step_abi.lib()
+    size = L.step_sum_slices_workspace(tokens, rows, width)
+    ws = _empty(size, dtype=torch.uint8, device=device)
+    step_abi.check(L.step_sum_slices(
+        indices.data_ptr(), _IDS[indices.dtype], tokens, flat.data_ptr(), _FLOATS[dtype], rows, width, stride, scale,
+        out_ids.data_ptr(), out.data_ptr(), count.data_ptr(), ws.data_ptr(), size, _stream_of(index)), "sum_slices")
+    n = count.item()
+    return out_ids[:n], out[:n].view((n,) + shape)
 
 
 class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, sparse):
         ctx.save_for_backward(ids)
-        ctx.rows, ctx.scale, ctx.sparse = weight.shape[0], scale, sparse
         ctx.set_materialize_grads(False)
+        ctx.call = (weight.shape[0], scale, sparse)
         return _lookup(ids, weight, scale)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
-        if grad is None or not ctx.needs_input_grad[1]:
+        if grad is None:
             return None, None, None, None
+        rows, scale, sparse = ctx.call
         ids, = ctx.saved_tensors
-        if not ctx.sparse:
-            return None, _gradient(grad, ids, ctx.rows, ctx.scale), None, None
+        if grad.requires_grad:
+            return None, _EmbeddingGradient.apply(grad, ids, rows, scale), None, None
+        if not sparse:
+            return None, _gradient(grad, ids, rows, scale), None, None
         if torch.cuda.is_current_stream_capturing():
             _refuse("embedding: the size of a sparse gradient depends on the data: it cannot be captured into a graph")
-        index, values = _sum_slices(grad.reshape(ids.numel(), grad.shape[-1]), ids.reshape(-1), ctx.rows, ctx.scale)
-        return None, torch.sparse_coo_tensor(index.long().unsqueeze(0), values, (ctx.rows, grad.shape[-1]),
+        index, values = _sum_slices(grad.reshape(ids.numel(), grad.shape[-1]), ids.reshape(-1), rows, scale)
+        return None, torch.sparse_coo_tensor(index.long().unsqueeze(0), values, (rows, grad.shape[-1]),
                                              is_coalesced=True, check_invariants=False), None, None
+
+
+class _EmbeddingGradient(torch.autograd.Function):
+    """The gradient as a function of its own, for gradients of gradients: it is linear, and its transpose the lookup."""
+
+    @staticmethod
+    def forward(ctx, grad, ids, rows, scale):
+        ctx.save_for_backward(ids)
+        ctx.scale = scale
+        return _gradient(grad, ids, rows, scale)
+
+    @staticmethod
+    def backward(ctx, grad):
+        ids, = ctx.saved_tensors
+        return embedding(ids, grad, ctx.scale), None, None, None
 
 
 def embedding(ids, weight, scale=1.0, sparse=False):
@@ -234,10 +256,9 @@ def embedding(ids, weight, scale=1.0, sparse=False):
     _same_device(what, ids, weight)
     if weight.dim() != 2:
         _refuse("%s: a table of shape %s; it has two dimensions", what, tuple(weight.shape))
-    scale = float(scale)
-    if torch.is_grad_enabled() and weight.requires_grad:
-        return _Embedding.apply(ids, weight, scale, bool(sparse))
-    return _lookup(ids, weight, scale)
+    if weight.requires_grad and torch.is_grad_enabled():
+        return _Embedding.apply(ids, weight, float(scale), bool(sparse))
+    return _lookup(ids, weight, float(scale))
 
 
 # The quintic whose five steps bring every singular value between 0.003 and 1 to within 0.7 .. 1.2.
@@ -287,17 +308,19 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
         _refuse("%s: a result of type %s", what, dtype)
     table = _coefficients(coefficients, steps, what)
     precise = dtype == torch.float32 if precise is None else bool(precise)
+    index = update.get_device()
+    if index != _current_device():
+        return _on_device(orthogonalize, update, update, steps, coefficients, eps, dtype, precise)
     update = update.detach().contiguous()
-    out = torch.empty(update.shape, dtype=dtype, device=update.device)
+    out = _empty(update.shape, dtype=dtype, device=update.device)
     rows, cols = update.shape[-2:]
     count = update.numel() // (rows * cols) if update.numel() else 0
     one = step_abi.Matrix(update.data_ptr(), None, out.data_ptr(), rows, cols, count, 0.0)
-    L = step_abi.lib()
-    with _on(update.device) as stream:
-        size = L.step_orthogonalize_workspace(one, 1, precise)
-        ws = _workspace(size, update.device)
-        step_abi.check(L.step_orthogonalize(one, 1, _FLOATS[update.dtype], _FLOATS[dtype], precise, steps, table,
-                                            float(eps), ws.data_ptr(), size, stream), what)
+    L = step_abi._lib or step_abi.lib()
+    size = L.step_orthogonalize_workspace(one, 1, precise)
+    ws = _empty(size, dtype=torch.uint8, device=update.device)
+    step_abi.check(L.step_orthogonalize(one, 1, _FLOATS[update.dtype], _FLOATS[dtype], precise, steps, table, float(eps),
+                                        ws.data_ptr(), size, _stream_of(index)), what)
     return out
 
 
@@ -359,7 +382,10 @@ class Muon(torch.optim.Optimizer):
                 if p.grad is not None:
                     alike.setdefault((p.device, p.dtype), []).append(p)
             for (device, dtype), params in alike.items():
-                self._step(group, device, dtype, params)
+                if device.type != "cuda":
+                    _refuse("Muon: a weight on %s; there are GPU kernels only", device)
+                with torch.cuda.device(device):
+                    self._step(group, device, dtype, params)
         return loss
 
     def _step(self, group, device, dtype, params):
@@ -370,7 +396,7 @@ class Muon(torch.optim.Optimizer):
             g = p.grad
             if g.is_sparse:
                 _refuse("Muon: a sparse gradient; it takes matrices with dense ones")
-            if not p.is_cuda or g.dtype != dtype or g.device != device:
+            if g.dtype != dtype or g.device != device:
                 _refuse("Muon: a weight of type %s on %s with a gradient of type %s on %s", dtype, device, g.dtype, g.device)
             state = self.state[p]
             m = state.get("momentum_buffer")
@@ -391,14 +417,13 @@ class Muon(torch.optim.Optimizer):
             row.rate = group["lr"] * (rule * math.sqrt(max(rows, cols)) if rule else math.sqrt(max(1.0, rows / cols)) if cols else 0.0)
         steps = group["steps"]
         precise = dtype == torch.float32 if group["precise"] is None else bool(group["precise"])
-        L = step_abi.lib()
-        with _on(device) as stream:
-            size = L.step_orthogonalize_workspace(table, len(params), precise)
-            ws = _workspace(size, device)
-            step_abi.check(L.step_muon(
-                table, len(params), _FLOATS[dtype], precise, steps, _coefficients(group["coefficients"], steps, "Muon"),
-                group["eps"], group["momentum"], bool(group["nesterov"]), 1.0 - group["lr"] * group["weight_decay"],
-                ws.data_ptr(), size, stream), "Muon.step")
+        L = step_abi._lib or step_abi.lib()
+        size = L.step_orthogonalize_workspace(table, len(params), precise)
+        ws = _empty(size, dtype=torch.uint8, device=device)
+        step_abi.check(L.step_muon(
+            table, len(params), _FLOATS[dtype], precise, steps, _coefficients(group["coefficients"], steps, "Muon"),
+            group["eps"], group["momentum"], bool(group["nesterov"]), 1.0 - group["lr"] * group["weight_decay"],
+            ws.data_ptr(), size, _stream_of(device.index)), "Muon.step")
         for p, w in moved:
             p.copy_(w)
 

@@ -360,3 +360,19 @@ def test_sparse_gradients_through_the_exchange(ranks):
     for w in weights:
         assert torch.equal(w, weights[0])
     assert bool(((weights[0].detach().double().cpu() - exact).abs() <= bound).all())
+
+
+def test_gradient_of_the_gradient():
+    """A penalty on the gradient of what the lookup feeds: the gradient is linear, its own gradient the lookup."""
+    ids = make_ids(60, 40, 12, "padded", torch.int64)
+    weight = values(61, 12, 10).requires_grad_(True)
+    mix = values(62, 40, 10).requires_grad_(True)
+    out = mpi.embedding(ids, weight, scale=2.0)
+    first, = torch.autograd.grad((out * mix).sum(), weight, create_graph=True)
+    first.square().sum().backward()
+    mirror_w, mirror_m = weight.detach().double().cpu().requires_grad_(True), mix.detach().double().cpu().requires_grad_(True)
+    inside = ids.cpu() >= 0
+    picked = torch.zeros(40, 10, dtype=torch.float64).index_put((inside,), 2.0 * mirror_w[ids.cpu()[inside]])
+    want, = torch.autograd.grad((picked * mirror_m).sum(), mirror_w, create_graph=True)
+    want.square().sum().backward()
+    assert torch.allclose(mix.grad.double().cpu(), mirror_m.grad, rtol=40 * U, atol=40 * U * float(mirror_m.grad.abs().max()))
