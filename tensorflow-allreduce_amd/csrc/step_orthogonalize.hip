@@ -3,7 +3,7 @@
 //
 // Mathematics. With U an m x n update (m <= n; a tall one is taken transposed),
 //   X_0 = U / (|U|_F + eps)
-//   X_k+1 = a X_k + (b A + c A A) X_k,   A = X_k X_k^T
+//   X_k+1 = (a I + b A + c A A) X_k,   A = X_k X_k^T
 // every singular value of X runs through the same odd polynomial and is brought
 // near 1 while the singular vectors stay. Three products per step: A and its
 // square are symmetric, so only the tiles on and below the diagonal are computed
@@ -14,7 +14,7 @@
 // sums. fp16 and not bfloat16: the iterates are bounded by about 1.2, so a fixed
 // power of two (kScaleX, kScaleA, kScaleB) keeps them inside fp16's range, and its
 // three more bits make every rounding eight times smaller. What is rounded off X
-// is kept: X = hi + lo / 2048 in two fp16 planes, and the linear term a X uses
+// is kept: X = hi + lo / 2048 in two fp16 planes, and the linear term a X counts
 // both. Without that, rounding noise in the directions that U hardly has grows by
 // a factor of a = 3.4 per step (485 in five), until it is 14 % of the result for
 // an update of rank one, and with it 0.03 to 0.2 % whatever the rank.
@@ -288,7 +288,8 @@ __global__ void __launch_bounds__(256) first_kernel(Segments segments, MomentumR
 
 // ---- products -----------------------------------------------------------------------
 
-// A = X X^T; B = b A + c A A; the next X and Y; the last X, to the caller.
+// A = X X^T; B = a I + b A + c A A; the next X = B X and its Y; the last X, to the caller. The linear term is on B's
+// diagonal, so that the products add it: no pass reads X for it, but the low plane where they do not.
 enum Kind { GRAM, SQUARE, APPLY, LAST };
 
 // Moves 16 bytes per lane from global memory into LDS at base + 16 * lane, without registers in between.
@@ -298,9 +299,16 @@ __device__ __forceinline__ void load_to_lds(const void* from, void* base) {
                                    16, 0, 0);
 }
 
+// Which row of a wave's part of a tile lane r of 16 reads for piece x. In pairs, so that the four rows of a result that a
+// lane holds of piece 2 k and the four of piece 2 k + 1 are eight in a row: 16 bytes of what is stored by columns.
+template <bool PAIRS> __device__ __forceinline__ uint32_t row_of_piece(uint32_t x, uint32_t r) {
+  return PAIRS ? x / 2 * 32 + r / 4 * 8 + x % 2 * 4 + r % 4 : x * 16 + r;
+}
 // A row of a stage is 64 halves: 8 chunks of 16 bytes, whose order depends on the row so that the 16 lanes that read one
-// chunk index of 16 rows touch different banks (no conflicts measured).
-__device__ __forceinline__ uint32_t chunk_place(uint32_t row, uint32_t chunk) { return chunk ^ ((row >> 1) & 7); }
+// chunk index of a piece's rows touch different banks (no conflicts measured).
+template <bool PAIRS> __device__ __forceinline__ uint32_t chunk_place(uint32_t row, uint32_t chunk) {
+  return chunk ^ (PAIRS ? (row >> 1 & 1) | (row >> 3 & 3) << 1 : row >> 1 & 7);
+}
 
 // Asks the compiler to mix the LDS reads and global loads of a half step among its products instead of putting them first.
 template <int READS, int PRODUCTS, int LOADS> __device__ __forceinline__ void interleave() {
@@ -397,6 +405,8 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   static_assert(SIDE * 8 % THREADS == 0, "a load belongs to one operand");
   static_assert(KS == 1 || (KS == 2 && FN % 2 == 0), "");
   constexpr int EN = FN / KS;                               // pieces across that a wave finishes
+  constexpr bool PAIR_P = FM % 2 == 0, PAIR_Q = EN % 2 == 0;  // rows, columns of pieces are taken in pairs
+  constexpr int DOWN = PAIR_P ? 2 : 1, ACROSS = PAIR_Q ? 2 : 1;
   constexpr int STAGED = STAGES * KS * SUB, SUMS = KS == 1 ? 0 : KS * SIDE * SIDE * 2;
   __shared__ _Float16 lds[STAGED > SUMS ? STAGED : SUMS];
 
@@ -425,7 +435,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
     const uint32_t chunk = k * THREADS + threadIdx.x % THREADS, row = chunk / 8;
     const bool second = k >= PER_OPERAND;
     const uint32_t r = second ? row - SIDE : row, end = second ? rows_q - j0 - 1 : m - i0 - 1;
-    offset[k] = ((r < end ? r : end) * (depth / 8) + chunk_place(row, chunk % 8)) * 16;
+    offset[k] = ((r < end ? r : end) * (depth / 8) + (second ? chunk_place<PAIR_Q>(r, chunk % 8) : chunk_place<PAIR_P>(r, chunk % 8))) * 16;
   }
   const uint64_t row_p = static_cast<uint64_t>(i0) * depth * 2, row_q = static_cast<uint64_t>(j0) * depth * 2;
   const uint64_t y_hi = p.y_hi + from * p.y_hi_step, y_lo = p.y_lo + from * p.y_lo_step;
@@ -453,13 +463,13 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
     for (int h = 0; h < PLANES; h++) {
 #pragma unroll
       for (int x = 0; x < FM; x++) {
-        const uint32_t row = wi + x * 16 + lane % 16;
-        fp[s][h][x] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + row) * 64 + chunk_place(row, chunk) * 8);
+        const uint32_t row = wi + row_of_piece<PAIR_P>(x, lane % 16);
+        fp[s][h][x] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + row) * 64 + chunk_place<PAIR_P>(row, chunk) * 8);
       }
 #pragma unroll
       for (int y = 0; y < FN; y++) {
-        const uint32_t row = SIDE + wj + y * 16 + lane % 16;
-        fq[s][h][y] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + row) * 64 + chunk_place(row, chunk) * 8);
+        const uint32_t row = wj + row_of_piece<PAIR_Q>(y, lane % 16);
+        fq[s][h][y] = *reinterpret_cast<const half8*>(stage + (h * 2 * SIDE + SIDE + row) * 64 + chunk_place<PAIR_Q>(row, chunk) * 8);
       }
     }
   };
@@ -538,30 +548,34 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
       }
   }
 
-  // A lane holds rows 4 (lane / 16) + 0..3 and column lane % 16 of every 16 x 16 piece: 8 bytes of what is stored by
-  // columns. Exchanged among four lanes it is 8 bytes of what is stored by rows. Addresses: the wave's corner, the same
-  // for all its lanes, then 32 bits for a lane's place in it.
-  const uint64_t old_hi_at = FROM_Y ? y_hi : p.a_hi, old_lo_at = FROM_Y ? y_lo : p.a_lo;
+  // A lane holds rows 4 (lane / 16) + 0..3 and column lane % 16 of every 16 x 16 piece: of a pair of them 16 bytes of what
+  // is stored by columns. Exchanged among four lanes it is 16 bytes of what is stored by rows. Addresses: the wave's
+  // corner, the same for all its lanes, then 32 bits for a lane's place in it.
+  const uint64_t old_hi_at = p.a_hi, old_lo_at = FROM_Y ? y_lo : p.a_lo;
   const uint64_t col_hi_at = KIND == APPLY ? p.y_hi + (from ^ 1) * p.y_hi_step : KIND == GRAM ? p.a_hi : p.b_hi;
   const uint64_t col_lo_at = KIND == APPLY ? p.y_lo + (from ^ 1) * p.y_lo_step : KIND == GRAM ? p.a_lo : p.b_lo;
   const uint64_t row_hi_at = KIND == APPLY ? p.x_hi : col_hi_at, row_lo_at = KIND == APPLY ? p.x_lo : col_lo_at;
   const uint32_t row_length = FROM_Y ? n : m;
   const uint64_t corner_i = i0 + wi, corner_j = j0 + wj + ey * 16;
   const uint64_t col_corner = (corner_j * m + corner_i) * 2, row_corner = (corner_i * row_length + corner_j) * 2;
-  const uint32_t col_lane = (lane % 16 * m + lane / 16 * 4) * 2;
-  const uint32_t row_lane = ((lane / 16 * 4 + lane % 4) * row_length + lane % 16 / 4 * 4) * 2;
-  // The linear term's operand is fetched some rows of pieces ahead of its use: the stores may not pass the loads.
-  constexpr int AHEAD = FM < 4 ? FM : 4;
-  const bool with_low = KIND != GRAM && (SPLIT || (FROM_Y && low_in));
-  half4 old_hi[AHEAD][EN], old_lo[AHEAD][EN];
-  auto fetch = [&](int x) {
-    if (KIND == GRAM || corner_i + x * 16 >= m) return;
+  // a lane's first row and column by columns; its row and first column by rows
+  const uint32_t col_i = lane / 16 * (4 * DOWN), col_j = row_of_piece<PAIR_Q>(0, lane % 16);
+  const uint32_t row_i = lane / 16 * (4 * DOWN) + lane % 4, row_j = lane % 16 / 4 * (4 * ACROSS);
+  const uint32_t col_lane = (col_j * m + col_i) * 2, row_lane = (row_i * row_length + row_j) * 2;
+  // What the result is made from is fetched some rows of pieces ahead of its use: the stores may not pass the loads.
+  constexpr int SETS = FM / DOWN, AHEAD = SETS < 3 ? SETS : 3;
+  const bool with_hi = KIND == SQUARE, with_low = KIND == SQUARE ? SPLIT : !SPLIT && FROM_Y && low_in;
+  typedef std::conditional_t<PAIR_P, half8, half4> Down;
+  typedef std::conditional_t<PAIR_Q, half8, half4> Across;
+  Down old_hi[AHEAD][EN], old_lo[AHEAD][EN];
+  auto fetch = [&](int set) {
+    if (KIND == GRAM || corner_i + set * 16 * DOWN >= m) return;
 #pragma unroll
     for (int y = 0; y < EN; y++) {
-      if (corner_j + y * 16 >= rows_q) break;
-      const char* from_col = at + col_corner + (static_cast<uint64_t>(y) * 16 * m + x * 16) * 2;
-      old_hi[x % AHEAD][y] = *reinterpret_cast<const half4*>(from_col + old_hi_at + col_lane);
-      if (with_low) old_lo[x % AHEAD][y] = *reinterpret_cast<const half4*>(from_col + old_lo_at + col_lane);
+      if (corner_j + y / ACROSS * 16 * ACROSS >= rows_q) break;
+      const char* from_col = at + col_corner + (static_cast<uint64_t>(y / ACROSS * 16 * ACROSS + y % ACROSS * 4) * m + set * 16 * DOWN) * 2;
+      if (with_hi) old_hi[set % AHEAD][y] = *reinterpret_cast<const Down*>(from_col + old_hi_at + col_lane);
+      if (with_low) old_lo[set % AHEAD][y] = *reinterpret_cast<const Down*>(from_col + old_lo_at + col_lane);
     }
   };
   Target t = {};
@@ -579,53 +593,81 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   auto finish = [&](auto type) {
     typedef decltype(type) T;
 #pragma unroll
-    for (int x = 0; x < AHEAD - 1; x++) fetch(x);
+    for (int set = 0; set < AHEAD - 1; set++) fetch(set);
 #pragma unroll
-    for (int x = 0; x < FM; x++) {
-      if (x + AHEAD - 1 < FM) fetch(x + AHEAD - 1);
-      if (corner_i + x * 16 >= m) break;
+    for (int set = 0; set < SETS; set++) {
+      if (set + AHEAD - 1 < SETS) fetch(set + AHEAD - 1);
+      if (corner_i + set * 16 * DOWN >= m) break;
 #pragma unroll
-      for (int y = 0; y < EN; y++) {
-        if (corner_j + y * 16 >= rows_q) break;
-        float4v v;
+      for (int y0 = 0; y0 < EN; y0 += ACROSS) {
+        if (corner_j + y0 * 16 >= rows_q) break;
+        Across row_hi[DOWN], row_lo[DOWN];
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (KIND == GRAM) {
-            v[e] = sum[x][y][e] * (kScaleA / (kScaleX * kScaleX));
-          } else {
-            float old = static_cast<float>(old_hi[x % AHEAD][y][e]);
-            if (with_low) old += static_cast<float>(old_lo[x % AHEAD][y][e]) * (1.f / kScaleLow);
-            v[e] = FROM_Y ? a * old + sum[x][y][e] * (1.f / kScaleB)
-                          : b * (kScaleB / kScaleA) * old + c * (kScaleB / kScaleA / kScaleA) * sum[x][y][e];
+        for (int dy = 0; dy < ACROSS; dy++) {
+          const int y = y0 + dy;
+          Down hi, lo;
+#pragma unroll
+          for (int dx = 0; dx < DOWN; dx++) {
+            float4v v = sum[set * DOWN + dx][y];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+              if (KIND == GRAM) {
+                v[e] *= kScaleA / (kScaleX * kScaleX);
+              } else if (KIND == SQUARE) {
+                float old = static_cast<float>(old_hi[set % AHEAD][y][dx * 4 + e]);
+                if (with_low) old += static_cast<float>(old_lo[set % AHEAD][y][dx * 4 + e]) * (1.f / kScaleLow);
+                v[e] = b * (kScaleB / kScaleA) * old + c * (kScaleB / kScaleA / kScaleA) * v[e];
+                if (corner_i + set * 16 * DOWN + col_i + dx * 4 + e == corner_j + y0 * 16 + dy * 4 + col_j) v[e] += a * kScaleB;
+              } else {
+                v[e] *= 1.f / kScaleB;
+                if (with_low) v[e] += a * (1.f / kScaleLow) * static_cast<float>(old_lo[set % AHEAD][y][dx * 4 + e]);
+              }
+            }
+            if constexpr (KIND == LAST) {
+              v = v * (1.f / kScaleX);
+              if (!tall) v = transpose4(v);
+              const uint64_t i = corner_i + set * 16 * DOWN + dx * 4 + (tall ? col_i : row_i);
+              const uint64_t j = corner_j + y0 * 16 + dy * 4 + (tall ? col_j : row_j);
+              const uint64_t r = tall ? j : i, col = tall ? i : j;
+              if (r < t.rows && col < t.cols) {
+                T* to = static_cast<T*>(t.out) + r * t.cols + col;
+                if (muon) v = keep * load4(to, t.cols - col) - t.rate * v;
+                store4(to, v, t.cols - col);
+              }
+            } else {
+              half4 h, l;
+#pragma unroll
+              for (int e = 0; e < 4; e++) {
+                _Float16 one, rest;
+                split_value(v[e], &one, &rest);
+                h[e] = hi[dx * 4 + e] = one;
+                l[e] = lo[dx * 4 + e] = rest;
+              }
+              const half4 th = transpose4(h);
+#pragma unroll
+              for (int e = 0; e < 4; e++) row_hi[dx][dy * 4 + e] = th[e];
+              if (SPLIT) {
+                const half4 tl = transpose4(l);
+#pragma unroll
+                for (int e = 0; e < 4; e++) row_lo[dx][dy * 4 + e] = tl[e];
+              }
+            }
+          }
+          if constexpr (KIND != LAST) {
+            if (KIND == APPLY || ti != tj) {               // Y; the mirror image of a tile off the diagonal
+              char* to_col = at + col_corner + (static_cast<uint64_t>(y0 * 16 + dy * 4) * m + set * 16 * DOWN) * 2;
+              *reinterpret_cast<Down*>(to_col + col_hi_at + col_lane) = hi;
+              if (SPLIT ? true : KIND == APPLY && low_out) *reinterpret_cast<Down*>(to_col + col_lo_at + col_lane) = lo;
+            }
           }
         }
-        if constexpr (KIND == LAST) {
-          v = v * (1.f / kScaleX);
-          if (!tall) v = transpose4(v);
-          const uint64_t i = corner_i + x * 16 + lane / 16 * 4, j = corner_j + y * 16 + lane % 16;
-          const uint64_t r = tall ? j : i + lane % 4, col = tall ? i : j / 4 * 4;
-          if (r < t.rows && col < t.cols) {
-            T* to = static_cast<T*>(t.out) + r * t.cols + col;
-            if (muon) v = keep * load4(to, t.cols - col) - t.rate * v;
-            store4(to, v, t.cols - col);
-          }
-        } else {
-          half4 hi, lo;
+        if constexpr (KIND != LAST) {
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            _Float16 h, l;
-            split_value(v[e], &h, &l);
-            hi[e] = h;
-            lo[e] = l;
+          for (int dx = 0; dx < DOWN; dx++) {
+            char* to_row = at + row_corner + (static_cast<uint64_t>(set * 16 * DOWN + dx * 4) * row_length + y0 * 16) * 2;
+            *reinterpret_cast<Across*>(to_row + row_hi_at + row_lane) = row_hi[dx];
+            if (SPLIT) *reinterpret_cast<Across*>(to_row + row_lo_at + row_lane) = row_lo[dx];
           }
-          char* to_col = at + col_corner + (static_cast<uint64_t>(y) * 16 * m + x * 16) * 2;
-          char* to_row = at + row_corner + (static_cast<uint64_t>(x) * 16 * row_length + y * 16) * 2;
-          if (KIND == APPLY || ti != tj) {                 // Y; the mirror image of a tile off the diagonal
-            *reinterpret_cast<half4*>(to_col + col_hi_at + col_lane) = hi;
-            if (SPLIT || (KIND == APPLY && low_out)) *reinterpret_cast<half4*>(to_col + col_lo_at + col_lane) = lo;
-          }
-          *reinterpret_cast<half4*>(to_row + row_hi_at + row_lane) = transpose4(hi);
-          if (SPLIT) *reinterpret_cast<half4*>(to_row + row_lo_at + row_lane) = transpose4(lo);
         }
       }
     }
@@ -774,8 +816,8 @@ void launch_product(const Groups& groups, uint32_t tiles, const Extra& targets, 
 
 // The tile size by what the launch would take with each. Large tiles read less per product but leave compute units idle
 // where there are few; the costs are those measured for one 1024 x 4096, 16 of 1024 x 1024, 4096 x 4096, 4096 x 16384 and
-// 8192 x 8192. Triangles: 4096 x 16384 half has 136 tiles of 256 (365 us), 253 of 192 (290 us), 528 of 128 (382 us); 1024 x
-// 4096 has 36 of 128 (41 us) and 136 of 64 (15 us).
+// 8192 x 8192. The Gram matrix of 4096 x 16384 has 136 tiles of 256 (326 us), 253 of 192 (256 us) or 528 of 128 (355 us), that of
+// 1024 x 2752 has 36 of 128 (33 us) or 136 of 64 (17 us).
 template <Kind KIND, bool SPLIT, typename Extra>
 void product(const Layout& l, const Extra& targets, char* ws, int from, int low_in, int low_out, const float* coefficients,
              hipStream_t stream) {
@@ -791,15 +833,15 @@ void product(const Layout& l, const Extra& targets, char* ws, int from, int low_
     launch_product<__VA_ARGS__, KIND, SPLIT>(g, t, targets, ws, from, low_in, low_out, coefficients, stream);        \
   }
   if constexpr (SPLIT) {
-    const double large = cut<KIND>(groups, l.counts, 128, Cost{1.1, KIND == LAST ? 18. : KIND == APPLY ? 24. : 10., 1}, &tiles);
-    const double small = cut<KIND>(groups, l.counts, 64, Cost{0.47, SQUARES ? 5.8 : 3.3, 1}, &tiles);
+    const double large = cut<KIND>(groups, l.counts, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
+    const double small = cut<KIND>(groups, l.counts, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
     if (large < small) go(STEP_PRODUCT(128, 2, 4, 1, 2), 128);
     else go(STEP_PRODUCT(64, 2, 2, 2, 2), 64);
   } else {
-    const double t256 = cut<KIND>(groups, l.counts, 256, Cost{1.42, KIND == LAST ? 36. : KIND == APPLY ? 70. : 10., 1}, &tiles);
-    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, l.counts, 192, Cost{1.0, 7., 1}, &tiles);
-    const double t128 = cut<KIND>(groups, l.counts, 128, Cost{1.0, KIND == LAST ? 16. : KIND == APPLY ? 20. : 5., 2}, &tiles);
-    const double t64 = cut<KIND>(groups, l.counts, 64, Cost{0.17, SQUARES ? 4.3 : 2.7, 1}, &tiles);
+    const double t256 = cut<KIND>(groups, l.counts, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? 22. : KIND == APPLY ? 28. : 10., 1}, &tiles);
+    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, l.counts, 192, Cost{0.98, 5., 1}, &tiles);
+    const double t128 = cut<KIND>(groups, l.counts, 128, Cost{0.98, KIND == LAST ? 8. : KIND == APPLY ? 10. : 4., 2}, &tiles);
+    const double t64 = cut<KIND>(groups, l.counts, 64, Cost{0.17, 3.5, 1}, &tiles);
     if (t64 <= std::min(std::min(t256, t192), t128)) go(STEP_PRODUCT(64, 2, 2, 2, 4), 64);
     else if (t128 <= std::min(t256, t192)) go(STEP_PRODUCT(128, 2, 2, 1, 2), 128);
     else if (t256 <= t192) go(STEP_PRODUCT(256, 2, 4, 1, 2), 256);
