@@ -94,7 +94,7 @@ struct Group {
   uint32_t m, n;          // padded
   uint32_t first_tile;    // of the launch
   uint32_t tiles;         // of one matrix
-  uint32_t first_matrix;  // of the round
+  uint32_t count, first_matrix;  // its matrices of the round
 };
 struct Groups {
   Group at[kMostGroups];
@@ -410,11 +410,13 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   constexpr int STAGED = STAGES * KS * SUB, SUMS = KS == 1 ? 0 : KS * SIDE * SIDE * 2;
   __shared__ _Float16 lds[STAGED > SUMS ? STAGED : SUMS];
 
-  // Workgroups are dealt to the eight chiplets in turn: give each chiplet, and its cache, neighbouring tiles.
-  const uint32_t share = gridDim.x / 8, spare = gridDim.x % 8, chiplet = blockIdx.x % 8;
-  const uint32_t of_all = chiplet * share + (chiplet < spare ? chiplet : spare) + blockIdx.x / 8;
-  const Group& g = groups.at[find(groups, of_all)];
-  const uint32_t m = g.m, n = g.n, matrix = (of_all - g.first_tile) / g.tiles, tile = (of_all - g.first_tile) % g.tiles;
+  // Workgroups are dealt to the eight chiplets in turn: give each chiplet, and its cache, an eighth of every group's tiles
+  // that are neighbours.
+  const Group& g = groups.at[find(groups, blockIdx.x)];
+  const uint32_t m = g.m, n = g.n, in_group = blockIdx.x - g.first_tile, of_group = g.tiles * g.count;
+  const uint32_t share = of_group / 8, spare = of_group % 8, chiplet = in_group % 8;
+  const uint32_t number = chiplet * share + (chiplet < spare ? chiplet : spare) + in_group / 8;
+  const uint32_t matrix = number / g.tiles, tile = number % g.tiles;
   const Planes p = planes_of(m, n, SPLIT);
   char* at = ws + g.base + matrix * p.bytes;
   uint32_t ti, tj;
@@ -582,9 +584,9 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   bool tall = false, muon = false;
   float keep = 0.f;
   if constexpr (KIND == LAST) {
-    const uint32_t number = g.first_matrix + matrix;
-    t = targets.at[find(targets, number)];
-    const uint64_t skip = static_cast<uint64_t>(number - t.first_tile) * t.rows * t.cols;
+    const uint32_t of_round = g.first_matrix + matrix;
+    t = targets.at[find(targets, of_round)];
+    const uint64_t skip = static_cast<uint64_t>(of_round - t.first_tile) * t.rows * t.cols;
     t.out = static_cast<char*>(t.out) + skip * (targets.type == STEP_F32 ? 4 : 2);
     tall = t.rows > t.cols;
     muon = targets.muon;
@@ -734,7 +736,6 @@ int for_rounds(const step_matrix* list, size_t length, const Visit& visit) {
 // The workspace of one round: its matrices, one behind the other.
 struct Layout {
   Groups groups;
-  uint32_t counts[kMostGroups];  // matrices of a group
   uint64_t base[kMostItems];
   uint64_t bytes;
 };
@@ -749,10 +750,9 @@ Layout layout_for(const Item* items, int count, bool split) {
     l.base[k] = l.bytes;
     const int g = l.groups.count - 1;
     if (g >= 0 && l.groups.at[g].m == item.m && l.groups.at[g].n == item.n) {
-      l.counts[g] += static_cast<uint32_t>(item.count);
+      l.groups.at[g].count += static_cast<uint32_t>(item.count);
     } else {
-      l.groups.at[l.groups.count] = {l.bytes, item.m, item.n, 0, 0, number};
-      l.counts[l.groups.count++] = static_cast<uint32_t>(item.count);
+      l.groups.at[l.groups.count++] = {l.bytes, item.m, item.n, 0, 0, static_cast<uint32_t>(item.count), number};
     }
     number += static_cast<uint32_t>(item.count);
     l.bytes += planes_of(item.m, item.n, split).bytes * item.count;
@@ -786,18 +786,19 @@ struct Cost {
 };
 constexpr uint32_t kUnits = 256;  // compute units
 
-// The tiles of side `side` of a product of every group, and about how long the launch takes.
-template <Kind KIND> double cut(Groups& groups, const uint32_t* counts, uint32_t side, const Cost& cost, uint32_t* tiles) {
+// The tiles of side `side` of a product of every group, the deepest first, and about how long the launch takes.
+template <Kind KIND> double cut(Groups& groups, uint32_t side, const Cost& cost, uint32_t* tiles) {
   double work = 0, longest = 0;
   *tiles = 0;
+  std::stable_sort(groups.at, groups.at + groups.count, [](const Group& x, const Group& y) { return KIND == GRAM ? x.n > y.n : x.m > y.m; });
   for (int k = 0; k < groups.count; k++) {
     Group& g = groups.at[k];
     const uint32_t down = (g.m + side - 1) / side, across = (g.n + side - 1) / side;
     g.tiles = KIND == APPLY || KIND == LAST ? down * across : down * (down + 1) / 2;
     g.first_tile = *tiles;
-    *tiles += g.tiles * counts[k];
+    *tiles += g.tiles * g.count;
     const double one = (KIND == GRAM ? g.n : g.m) / 64 * cost.stage + cost.end;
-    work += one * g.tiles * counts[k];
+    work += one * g.tiles * g.count;
     longest = std::max(longest, one);
   }
   const uint32_t at_once = kUnits * cost.per_cu;
@@ -825,7 +826,7 @@ void product(const Layout& l, const Extra& targets, char* ws, int from, int low_
   Groups groups = l.groups;
   uint32_t tiles;
   auto go = [&](auto kernel, uint32_t side) {
-    cut<KIND>(groups, l.counts, side, Cost{0, 0, 1}, &tiles);
+    cut<KIND>(groups, side, Cost{0, 0, 1}, &tiles);
     kernel(groups, tiles);
   };
 #define STEP_PRODUCT(...)                                                                                            \
@@ -833,15 +834,15 @@ void product(const Layout& l, const Extra& targets, char* ws, int from, int low_
     launch_product<__VA_ARGS__, KIND, SPLIT>(g, t, targets, ws, from, low_in, low_out, coefficients, stream);        \
   }
   if constexpr (SPLIT) {
-    const double large = cut<KIND>(groups, l.counts, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
-    const double small = cut<KIND>(groups, l.counts, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
+    const double large = cut<KIND>(groups, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
+    const double small = cut<KIND>(groups, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
     if (large < small) go(STEP_PRODUCT(128, 2, 4, 1, 2), 128);
     else go(STEP_PRODUCT(64, 2, 2, 2, 2), 64);
   } else {
-    const double t256 = cut<KIND>(groups, l.counts, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? 22. : KIND == APPLY ? 28. : 10., 1}, &tiles);
-    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, l.counts, 192, Cost{0.98, 5., 1}, &tiles);
-    const double t128 = cut<KIND>(groups, l.counts, 128, Cost{0.98, KIND == LAST ? 8. : KIND == APPLY ? 10. : 4., 2}, &tiles);
-    const double t64 = cut<KIND>(groups, l.counts, 64, Cost{0.17, 3.5, 1}, &tiles);
+    const double t256 = cut<KIND>(groups, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? 22. : KIND == APPLY ? 28. : 10., 1}, &tiles);
+    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, 192, Cost{0.98, 5., 1}, &tiles);
+    const double t128 = cut<KIND>(groups, 128, Cost{0.98, KIND == LAST ? 8. : KIND == APPLY ? 10. : 4., 2}, &tiles);
+    const double t64 = cut<KIND>(groups, 64, Cost{0.17, 3.5, 1}, &tiles);
     if (t64 <= std::min(std::min(t256, t192), t128)) go(STEP_PRODUCT(64, 2, 2, 2, 4), 64);
     else if (t128 <= std::min(t256, t192)) go(STEP_PRODUCT(128, 2, 2, 1, 2), 128);
     else if (t256 <= t192) go(STEP_PRODUCT(256, 2, 4, 1, 2), 256);
