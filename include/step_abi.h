@@ -90,7 +90,8 @@ int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* val
  *
  * precise = 0: the products take fp16 operands (the rest of the iterate is kept
  * beside them): the result is 0.02 to 0.2 % off, about bfloat16's own rounding.
- * precise = 1: three products of split operands: about 1e-6 off. Iterates must
+ * precise = 1: three products of split operands: about 1e-6 off; a list whose
+ * matrices are all of at most 64 x 256 (or 256 x 64) always has these. Iterates must
  * stay below 64 in every entry and X X^T below 4, which coefficients that bring
  * singular values towards 1 see to. */
 typedef struct step_matrix {
@@ -102,7 +103,7 @@ typedef struct step_matrix {
   float rate;        /* step_muon: learning rate of this batch's matrices */
 } step_matrix;
 
-/* Bytes of workspace for a list: 0 if there is nothing to do. */
+/* Bytes of workspace for a list: 0 if none is needed. */
 size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int precise);
 int step_orthogonalize(const step_matrix* list, size_t length, int dtype, int out_dtype, int precise, int steps,
                        const float* coefficients, float eps, void* workspace, size_t workspace_bytes, void* stream);

@@ -683,10 +683,230 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   }
 }
 
+// ---- small matrices -----------------------------------------------------------------
+
+// Matrices of at most 64 x 256 (or the transposed) are a workgroup each, from the momentum to the result in one launch:
+// both forms of X, A and B stay in LDS, every operand split. What bounds them is the chain of barriers and LDS reads of a
+// step (about 2 us), where the launches of the products above take 15.
+constexpr uint32_t kSmallRows = 64, kSmallCols = 256, kSmallThreads = 512;
+
+struct SmallItem {
+  const void* grad;
+  float* momentum;
+  void* out;
+  uint32_t first_tile;  // its first matrix of the launch
+  uint16_t rows, cols;
+  float rate;
+};
+struct SmallItems {
+  SmallItem at[kMostItems];
+  int count;
+  int out_type, muon, steps;
+  float keep, eps;
+};
+struct Coefficients {
+  float at[3 * kMostSteps];
+};
+
+// Halves of a row of `length` (a multiple of 64) in LDS, its chunks of 16 bytes ordered by the row.
+__device__ __forceinline__ uint32_t small_place(uint32_t row, uint32_t col, uint32_t length) {
+  const uint32_t chunk = col / 8 ^ (length == 64 ? row >> 1 & 7 : row & 7);
+  return row * length + chunk * 8 + col % 8;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(kSmallThreads) small_kernel(SmallItems items, Coefficients coefficients, MomentumRule rule) {
+  __shared__ _Float16 x_hi[64 * N], x_lo[64 * N], y_hi[64 * N], y_lo[64 * N], s_hi[64 * 64], s_lo[64 * 64];
+  __shared__ double sums[kSmallThreads / 64];
+  const SmallItem& item = items.at[find(items, blockIdx.x)];
+  const uint32_t rows = item.rows, cols = item.cols;
+  const bool tall = rows > cols;
+  const uint64_t base = static_cast<uint64_t>(blockIdx.x - item.first_tile) * rows * cols;
+  const uint32_t lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+  const uint32_t strip = wave % 4 * 16, half = wave / 4 * 2;  // a wave's rows of A and B, and the first of its two pieces there
+
+  // the update, four elements of a row at a time, padded with zeros
+  constexpr int MOST = 64 * N / 4 / kSmallThreads;
+  const uint32_t per_row = (tall ? 64 : N) / 4;
+  float4v u[MOST];
+  double sum = 0;
+#pragma unroll
+  for (int k = 0; k < MOST; k++) {
+    const uint32_t v = k * kSmallThreads + threadIdx.x, r = v / per_row, c = v % per_row * 4;
+    u[k] = float4v{0, 0, 0, 0};
+    if (r >= rows || c >= cols) continue;
+    const uint64_t at = base + r * cols + c;
+    u[k] = load4(static_cast<const T*>(item.grad) + at, cols - c);
+    if (rule.use) {
+      F32* momentum = reinterpret_cast<F32*>(item.momentum) + at;
+      const float4v m = rule.momentum * load4(momentum, cols - c) + u[k];
+      store4(momentum, m, cols - c);
+      u[k] = rule.nesterov ? u[k] + rule.momentum * m : m;
+    }
+    for (int e = 0; e < 4; e++) {
+      if (c + e >= cols) u[k][e] = 0.f;
+      sum += static_cast<double>(u[k][e]) * u[k][e];
+    }
+  }
+  for (int step = 32; step; step /= 2) sum += __shfl_xor(sum, step);
+  if (lane == 0) sums[wave] = sum;
+  __syncthreads();
+  sum = 0;
+  for (int k = 0; k < static_cast<int>(kSmallThreads) / 64; k++) sum += sums[k];
+  const double scale = kScaleX / (sqrt(sum) + static_cast<double>(items.eps));
+#pragma unroll
+  for (int k = 0; k < MOST; k++) {
+    const uint32_t v = k * kSmallThreads + threadIdx.x, r = v / per_row, c = v % per_row * 4;
+    for (int e = 0; e < 4; e++) {
+      _Float16 hi, lo;
+      split_value(static_cast<float>(u[k][e] * scale), &hi, &lo);
+      const uint32_t i = tall ? c + e : r, j = tall ? r : c + e;
+      x_hi[small_place(i, j, N)] = hi;
+      x_lo[small_place(i, j, N)] = lo;
+      y_hi[small_place(j, i, 64)] = hi;
+      y_lo[small_place(j, i, 64)] = lo;
+    }
+  }
+
+  auto fragment = [&](const _Float16* from, uint32_t row, uint32_t k, uint32_t length) {
+    return *reinterpret_cast<const half8*>(from + small_place(row, k * 32 + lane / 16 * 8, length));
+  };
+  auto product = [](float4v& acc, float4v& low, half8 ph, half8 pl, half8 qh, half8 ql) {
+    acc = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, qh, acc, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(ph, ql, low, 0, 0, 0);
+    low = __builtin_amdgcn_mfma_f32_16x16x32_f16(pl, qh, low, 0, 0, 0);
+  };
+  // pieces of A and B, stored transposed, which they equal
+  auto put_square = [&](const float4v (&v)[2]) {
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      half4 hi, lo;
+      for (int e = 0; e < 4; e++) {
+        _Float16 h, l;
+        split_value(v[y][e], &h, &l);
+        hi[e] = h;
+        lo[e] = l;
+      }
+      const uint32_t to = small_place((half + y) * 16 + lane % 16, strip + lane / 16 * 4, 64);
+      *reinterpret_cast<half4*>(s_hi + to) = hi;
+      *reinterpret_cast<half4*>(s_lo + to) = lo;
+    }
+  };
+  constexpr int WAVES = kSmallThreads / 64, PN = N / 16 / WAVES;  // pieces across of a wave's columns of X
+  float4v next[4][PN];
+  for (int step = 0;; step++) {
+    const float a = coefficients.at[3 * step], b = coefficients.at[3 * step + 1], c = coefficients.at[3 * step + 2];
+    __syncthreads();
+    float4v acc[2] = {}, low[2] = {}, gram[2];
+#pragma unroll 2
+    for (uint32_t k = 0; k < N / 32; k++) {
+      const half8 ph = fragment(x_hi, strip + lane % 16, k, N), pl = fragment(x_lo, strip + lane % 16, k, N);
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+        product(acc[y], low[y], ph, pl, fragment(x_hi, (half + y) * 16 + lane % 16, k, N), fragment(x_lo, (half + y) * 16 + lane % 16, k, N));
+    }
+#pragma unroll
+    for (int y = 0; y < 2; y++) gram[y] = (acc[y] + low[y] * (1.f / kScaleLow)) * (kScaleA / (kScaleX * kScaleX));
+    put_square(gram);
+    __syncthreads();
+#pragma unroll
+    for (int y = 0; y < 2; y++) acc[y] = low[y] = float4v{0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++) {
+      const half8 ph = fragment(s_hi, strip + lane % 16, k, 64), pl = fragment(s_lo, strip + lane % 16, k, 64);
+#pragma unroll
+      for (int y = 0; y < 2; y++)
+        product(acc[y], low[y], ph, pl, fragment(s_hi, (half + y) * 16 + lane % 16, k, 64), fragment(s_lo, (half + y) * 16 + lane % 16, k, 64));
+    }
+#pragma unroll
+    for (int y = 0; y < 2; y++) {
+      gram[y] = b * (kScaleB / kScaleA) * gram[y] + c * (kScaleB / kScaleA / kScaleA) * (acc[y] + low[y] * (1.f / kScaleLow));
+      for (int e = 0; e < 4; e++)
+        if (strip + lane / 16 * 4 + e == (half + y) * 16 + lane % 16) gram[y][e] += a * kScaleB;
+    }
+    __syncthreads();  // every wave has read A
+    put_square(gram);
+    __syncthreads();
+    float4v next_low[4][PN];
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+      for (int y = 0; y < PN; y++) next[x][y] = next_low[x][y] = float4v{0, 0, 0, 0};
+#pragma unroll
+    for (uint32_t k = 0; k < 2; k++) {
+      half8 qh[PN], ql[PN];
+#pragma unroll
+      for (int y = 0; y < PN; y++) {
+        qh[y] = fragment(y_hi, wave * (N / WAVES) + y * 16 + lane % 16, k, 64);
+        ql[y] = fragment(y_lo, wave * (N / WAVES) + y * 16 + lane % 16, k, 64);
+      }
+#pragma unroll
+      for (int x = 0; x < 4; x++) {
+        const half8 ph = fragment(s_hi, x * 16 + lane % 16, k, 64), pl = fragment(s_lo, x * 16 + lane % 16, k, 64);
+#pragma unroll
+        for (int y = 0; y < PN; y++) product(next[x][y], next_low[x][y], ph, pl, qh[y], ql[y]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+      for (int y = 0; y < PN; y++) next[x][y] = (next[x][y] + next_low[x][y] * (1.f / kScaleLow)) * (1.f / kScaleB);
+    if (step + 1 == items.steps) break;
+    // a wave reads and writes rows of Y of its own; X was last read two barriers ago
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+      for (int y = 0; y < PN; y++) {
+        half4 hi, lo;
+        for (int e = 0; e < 4; e++) {
+          _Float16 h, l;
+          split_value(next[x][y][e], &h, &l);
+          hi[e] = h;
+          lo[e] = l;
+        }
+        const uint32_t j = wave * (N / WAVES) + y * 16;
+        const uint32_t by_col = small_place(j + lane % 16, x * 16 + lane / 16 * 4, 64);
+        const uint32_t by_row = small_place(x * 16 + lane / 16 * 4 + lane % 4, j + lane % 16 / 4 * 4, N);
+        *reinterpret_cast<half4*>(y_hi + by_col) = hi;
+        *reinterpret_cast<half4*>(y_lo + by_col) = lo;
+        *reinterpret_cast<half4*>(x_hi + by_row) = transpose4(hi);
+        *reinterpret_cast<half4*>(x_lo + by_row) = transpose4(lo);
+      }
+  }
+  auto finish = [&](auto type) {
+    typedef decltype(type) O;
+#pragma unroll
+    for (int x = 0; x < 4; x++)
+#pragma unroll
+      for (int y = 0; y < PN; y++) {
+        float4v v = next[x][y] * (1.f / kScaleX);
+        if (!tall) v = transpose4(v);
+        const uint32_t i = x * 16 + lane / 16 * 4 + (tall ? 0 : lane % 4);
+        const uint32_t j = wave * (N / WAVES) + y * 16 + (tall ? lane % 16 : lane % 16 / 4 * 4);
+        const uint32_t r = tall ? j : i, col = tall ? i : j;
+        if (r >= rows || col >= cols) continue;
+        O* to = static_cast<O*>(item.out) + base + r * cols + col;
+        if (items.muon) v = items.keep * load4(to, cols - col) - item.rate * v;
+        store4(to, v, cols - col);
+      }
+  };
+  if (items.out_type == STEP_F32) finish(F32());
+  else if (items.out_type == STEP_BF16) finish(BF16());
+  else finish(F16());
+}
+
 // ---- host side -----------------------------------------------------------------------
 
 // Elements of one round, beyond which more matrices fill the GPU no better and only ask for more workspace.
 constexpr uint64_t kRoundElements = 1ull << 26;
+
+// Whether all matrices of a list are small. Among larger ones they ride along in launches that are made anyway: of the
+// ResNet-50 set's 54 matrices 8 are small, and on their own they would take 98 us beside the 1370 of the whole step.
+bool all_small(const step_matrix* list, size_t length) {
+  for (size_t k = 0; k < length; k++)
+    if (std::min(list[k].rows, list[k].cols) > kSmallRows || std::max(list[k].rows, list[k].cols) > kSmallCols) return false;
+  return true;
+}
 
 struct Item {
   size_t matrix, first, count;  // matrices [first, first + count) of the caller's batch `matrix`
@@ -785,6 +1005,8 @@ struct Cost {
   uint32_t per_cu;
 };
 constexpr uint32_t kUnits = 256;  // compute units
+// Iterates of more elements (8 bytes of each are moved behind a product) do not stay in the 256 MB cache in front of HBM.
+constexpr uint64_t kNearElements = 1ull << 25;
 
 // The tiles of side `side` of a product of every group, the deepest first, and about how long the launch takes.
 template <Kind KIND> double cut(Groups& groups, uint32_t side, const Cost& cost, uint32_t* tiles) {
@@ -839,9 +1061,12 @@ void product(const Layout& l, const Extra& targets, char* ws, int from, int low_
     if (large < small) go(STEP_PRODUCT(128, 2, 4, 1, 2), 128);
     else go(STEP_PRODUCT(64, 2, 2, 2, 2), 64);
   } else {
-    const double t256 = cut<KIND>(groups, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? 22. : KIND == APPLY ? 28. : 10., 1}, &tiles);
+    uint64_t elements = 0;
+    for (int k = 0; k < groups.count; k++) elements += static_cast<uint64_t>(groups.at[k].m) * groups.at[k].n * groups.at[k].count;
+    const bool far = elements > kNearElements;
+    const double t256 = cut<KIND>(groups, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? (far ? 26. : 22.) : KIND == APPLY ? (far ? 35. : 28.) : 10., 1}, &tiles);
     const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, 192, Cost{0.98, 5., 1}, &tiles);
-    const double t128 = cut<KIND>(groups, 128, Cost{0.98, KIND == LAST ? 8. : KIND == APPLY ? 10. : 4., 2}, &tiles);
+    const double t128 = cut<KIND>(groups, 128, Cost{0.98, KIND == LAST ? (far ? 14. : 8.) : KIND == APPLY ? (far ? 20. : 10.) : 4., 2}, &tiles);
     const double t64 = cut<KIND>(groups, 64, Cost{0.17, 3.5, 1}, &tiles);
     if (t64 <= std::min(std::min(t256, t192), t128)) go(STEP_PRODUCT(64, 2, 2, 2, 4), 64);
     else if (t128 <= std::min(t256, t192)) go(STEP_PRODUCT(128, 2, 2, 1, 2), 128);
@@ -901,12 +1126,49 @@ int run_round(const step_matrix* list, const Item* items, int count, int dtype, 
   return launched();
 }
 
+// A list of small matrices, those of up to 64 x 128 apart: two workgroups of them fit a compute unit's LDS.
+int run_small(const step_matrix* list, size_t length, int dtype, int out_dtype, const Rule& rule, hipStream_t stream) {
+  bool any = false;
+  Coefficients coefficients;
+  memcpy(coefficients.at, rule.coefficients, sizeof(float) * 3 * rule.steps);
+  for (const uint32_t across : {128u, 256u}) {
+    SmallItems items;
+    items.out_type = out_dtype;
+    items.muon = rule.muon;
+    items.steps = rule.steps;
+    items.keep = rule.keep;
+    items.eps = rule.eps;
+    items.count = 0;
+    uint32_t matrices = 0;
+    auto flush = [&]() {
+      if (!items.count) return;
+      by_type(dtype, [&](auto type) {
+        typedef decltype(type) T;
+        if (across == 128) hipLaunchKernelGGL((small_kernel<T, 128>), dim3(matrices), dim3(kSmallThreads), 0, stream, items, coefficients, rule.momentum);
+        else hipLaunchKernelGGL((small_kernel<T, 256>), dim3(matrices), dim3(kSmallThreads), 0, stream, items, coefficients, rule.momentum);
+      });
+      any = true;
+      items.count = 0;
+      matrices = 0;
+    };
+    for (size_t k = 0; k < length; k++) {
+      const step_matrix& x = list[k];
+      if (x.rows == 0 || x.cols == 0 || x.count == 0 || (std::max(x.rows, x.cols) <= 128) != (across == 128)) continue;
+      if (items.count == kMostItems || x.count > kMostSize - matrices) flush();
+      items.at[items.count++] = {x.grad, x.momentum, x.out, matrices, static_cast<uint16_t>(x.rows), static_cast<uint16_t>(x.cols), x.rate};
+      matrices += static_cast<uint32_t>(x.count);
+    }
+    flush();
+  }
+  return any ? launched() : static_cast<int>(STEP_OK);
+}
+
 int run(const step_matrix* list, size_t length, int dtype, int out_dtype, int precise, const Rule& rule, void* workspace,
         size_t workspace_bytes, hipStream_t stream) {
   if (rule.steps < 1 || rule.steps > kMostSteps || !rule.coefficients) return STEP_ERR_ARGUMENT;
   const size_t need = step_orthogonalize_workspace(list, length, precise);
-  if (need == 0) return STEP_OK;
-  if (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
+  if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)) return STEP_ERR_ARGUMENT;
+  if (need == 0) return run_small(list, length, dtype, out_dtype, rule, stream);  // or nothing to do
   char* ws = static_cast<char*>(workspace);
   return for_rounds(list, length, [&](const Item* items, int count) {
     return precise ? run_round<true>(list, items, count, dtype, out_dtype, rule, ws, stream)
@@ -923,7 +1185,7 @@ extern "C" {
 
 size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int precise) {
   uint64_t most = 0;
-  if (length && !list) return 0;
+  if ((length && !list) || all_small(list, length)) return 0;
   for_rounds(list, length, [&](const Item* items, int count) {
     most = std::max(most, layout_for(items, count, precise != 0).bytes);
     return static_cast<int>(STEP_OK);

@@ -296,7 +296,8 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
                 of each iterate kept beside them: the result is 0.02 to 0.2 % off
                 (2-norm), whatever update's rank; bfloat16's own rounding is
                 0.17 %. True: products of split operands, three times the work:
-                about 1e-6 off. Default: True if the result is float32.
+                about 1e-6 off. Default: True if the result is float32. Matrices
+                of at most 64 x 256 (or the transposed) are always precise.
 
     An update with an infinity or NaN gives NaN."""
     what = "orthogonalize"

@@ -71,7 +71,7 @@ def gradient(seed, *shape, rank=8, noise=0.3, size=1e-4, dtype=torch.float32):
     return (size * (low + noise * torch.randn(*shape, generator=gen))).to(dtype).cuda()
 
 
-SHAPES = [(1, 1), (1, 100), (100, 1), (3, 5), (64, 64), (64, 128), (65, 63), (128, 128), (129, 500), (200, 130), (500, 129),
+SHAPES = [(1, 1), (1, 100), (64, 256), (250, 64), (33, 129), (64, 257), (100, 1), (3, 5), (64, 64), (64, 128), (65, 63), (128, 128), (129, 500), (200, 130), (500, 129),
           (1000, 1), (256, 1024), (777, 333), (1000, 1500), (2000, 130)]
 
 
@@ -192,17 +192,19 @@ def test_muon(dtype, options):
 
 
 def test_muon_with_many_matrices_of_many_shapes():
-    """More matrices than one launch carries, and as one list the same bits as one by one."""
+    """More matrices than one launch carries; as one list and one by one they differ by the split products' roundings only."""
     shapes = [(8 + 3 * (k % 30), 16 + 5 * (k % 17)) for k in range(130)]
     make = lambda: [torch.nn.Parameter(gradient(k, *s, size=1.0)) for k, s in enumerate(shapes)]  # noqa: E731
     together, apart = make(), make()
     for p, q in zip(together, apart):
         p.grad = q.grad = gradient(int(p.numel()), *p.shape)
+    start = [p.detach().clone() for p in together]
     mpi.Muon(together).step()
     for q in apart:
         mpi.Muon([q]).step()
-    for p, q in zip(together, apart):
-        assert torch.equal(p, q)
+    for p, q, w in zip(together, apart, start):
+        p, q = p.detach(), q.detach()
+        assert float((p - q).norm()) <= 2 * SPLIT * float((q - w).norm()) + 2.0 ** -22 * float(q.norm())
 
 
 def test_muon_strides_state_and_groups():

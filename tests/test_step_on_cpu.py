@@ -116,20 +116,22 @@ def test_orthogonalize_refuses_on_the_host():
     assert call(m=M(None, None, 4096, 100, 200, 3, 0)) == call(m=M(4096, None, None, 100, 200, 3, 0)) == 2
     assert call(m=M(4096, None, 4096, (1 << 20) + 1, 1, 1, 0)) == call(m=M(4096, None, 4096, 1 << 20, 1 << 20, 1, 0)) == 5
     assert lib.step_muon(M(4096, None, 4096, 100, 200, 3, 0), 1, 0, 0, 5, abc, 0.0, 0.9, 1, 1.0, 4096, size, None) == 2
-    for empty in (M(None, None, None, 0, 7, 3, 0), M(None, None, None, 7, 0, 3, 0), M(None, None, None, 7, 7, 0, 0)):
+    for empty in (M(None, None, None, 0, 700, 3, 0), M(None, None, None, 700, 0, 3, 0), M(None, None, None, 700, 700, 0, 0)):
         assert lib.step_orthogonalize_workspace(empty, 1, 0) == 0 and call(m=empty, ws=None, bytes=0) == 0
     # the workspace of a long list is that of its largest round, not of the whole list
     many = (M * 500)(*[M(4096, 4096, 4096, 4096, 4096, 1, 0.1) for _ in range(500)])
     assert lib.step_orthogonalize_workspace(many, 500, 0) < 6 << 30
-    assert lib.step_orthogonalize_workspace(M(4096, None, 4096, 64, 64, 10 ** 7, 0), 1, 0) < 4 << 30
+    assert lib.step_orthogonalize_workspace(M(4096, None, 4096, 65, 65, 10 ** 7, 0), 1, 0) < 4 << 30
+    # small ones need none
+    assert lib.step_orthogonalize_workspace(M(4096, None, 4096, 64, 256, 10 ** 7, 0), 1, 1) == 0
 
 
 def test_orthogonalize_assembly():
     text = _assembly(ORTHOGONALIZE)
     found = stale_selects(text)
     assert not found, "scalar selects on a stale condition code: %r" % (found[:5],)
-    kernels = kernels_in_scratch(text, ("norm_kernel", "first_kernel", "product_kernel"))
-    assert kernels["seen"] >= 21 and not kernels["scratch"], kernels
+    kernels = kernels_in_scratch(text, ("norm_kernel", "first_kernel", "product_kernel", "small_kernel"))
+    assert kernels["seen"] >= 37 and not kernels["scratch"], kernels
 
 
 def test_embedding_assembly():
