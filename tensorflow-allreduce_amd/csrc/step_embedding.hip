@@ -55,7 +55,7 @@ RowShape row_shape(size_t vectors) {
   RowShape s;
   s.chunks = static_cast<uint32_t>((vectors + 255) / 256);
   const size_t per_chunk = (vectors + s.chunks - 1) / s.chunks;
-  if (per_chunk <= 32) {
+  if (per_chunk <= 32) {  // else whole waves
     s.lanes = 1;
     while (s.lanes < per_chunk) s.lanes *= 2;
   } else {
@@ -185,8 +185,8 @@ __device__ __forceinline__ void wave_fence() {
 #if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
-#else
-  __syncthreads();
+#elif defined(STEP_WAVE_SHIM_H_)
+  step_wave_fence();
 #endif
 }
 
@@ -487,6 +487,15 @@ __global__ void __launch_bounds__(kSortThreads) number_runs_kernel(const uint32_
 
 // ---- sums ------------------------------------------------------------------------
 
+// What lane `from` (the same for all) holds, for every lane of its wave.
+__device__ __forceinline__ uint32_t broadcast(uint32_t x, uint32_t from) {
+#if defined(__HIP_DEVICE_COMPILE__)
+  return __builtin_amdgcn_readlane(x, from);
+#else
+  return __shfl(x, static_cast<int>(from));
+#endif
+}
+
 constexpr uint32_t kWindow = 8;     // places of the sorted order whose runs one row of lanes sums
 constexpr uint32_t kNoRow = 0xffffffffu;
 constexpr uint32_t kZeroRows = 64;  // rows of a workgroup that looks for empty ones
@@ -561,12 +570,65 @@ __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* ou
   if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
 }
 
+// The same where a row takes whole waves: the lanes of a wave look at 64 places at once and hand what they saw to all.
+// `mine`: whether this lane has columns; the others only look.
+template <typename T>
+__device__ __forceinline__ void sum_window_wide(const Sums& q, const T* values, T* out, uint32_t window, uint32_t vector, bool mine) {
+  constexpr int N = Vec<T>::kCount;
+  const uint32_t column = mine ? Access<T>::column(vector, q.width) : 0, lane = threadIdx.x % 64;
+  const uint64_t w0 = static_cast<uint64_t>(window) * kWindow;
+  float acc[N];
+  uint32_t open = kNoRow;
+  auto close = [&]() {
+    if (mine && open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+  };
+  for (uint64_t base = w0;; base += 64) {
+    const uint64_t i = base + lane;
+    const uint32_t row = i < q.tokens ? q.by.row_of[i] : kNoRow, order = i < q.tokens ? q.by.order[i] : 0;
+    const uint32_t before = i && i - 1 < q.tokens ? q.by.row_of[i - 1] : kNoRow;
+    const uint32_t ahead = i + q.piece < q.tokens ? q.by.row_of[i + q.piece] : kNoRow;
+    const bool starts = row != before, usable = base == w0 && lane < kWindow && row < q.rows && ahead != row;
+    // where runs of this window begin, and where there is nothing more to do: at a later window's run, at a dropped id
+    // or behind the last place, at a long run
+    const uint64_t begins = __ballot(starts && usable), stops = __ballot((starts || row == kNoRow) && !usable);
+    const uint32_t end = stops ? static_cast<uint32_t>(__builtin_ctzll(stops)) : 64;
+    uint32_t p = base == w0 ? (begins ? static_cast<uint32_t>(__builtin_ctzll(begins)) : 64) : 0;
+    if (p >= end) break;
+    auto add_rows = [&](auto rows) {
+      constexpr int U = decltype(rows)::value;
+      Vec<T> v[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const uint32_t from = broadcast(order, p + k);
+        if (mine) v[k] = Access<T>::load(values + from * q.stride + column, q.width);
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        if (begins >> (p + k) & 1) {
+          close();
+          open = broadcast(row, p + k);
+          for (int n = 0; n < N; n++) acc[n] = 0.f;
+        }
+        if (mine) add<T>(acc, v[k]);
+      }
+      p += U;
+    };
+    while (end - p >= 16) add_rows(std::integral_constant<int, 16>());
+    if (end - p >= 8) add_rows(std::integral_constant<int, 8>());
+    if (end - p >= 4) add_rows(std::integral_constant<int, 4>());
+    if (end - p >= 2) add_rows(std::integral_constant<int, 2>());
+    if (end - p >= 1) add_rows(std::integral_constant<int, 1>());
+    if (end < 64) break;
+  }
+  close();
+}
+
 // A long run's part: piece j holds the places j * piece .. of the sorted order. At most two long runs have a part in it,
 // that of its first place (parts[2 j]) and that of its last (parts[2 j + 1]).
-template <typename T, bool NUMBERED>
-__device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float* parts, uint32_t piece, uint32_t vector) {
+template <typename T, bool NUMBERED, bool WIDE>
+__device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float* parts, uint32_t piece, uint32_t vector, bool mine) {
   constexpr int N = Vec<T>::kCount;
-  const uint32_t column = Access<T>::column(vector, q.width);
+  const uint32_t column = mine ? Access<T>::column(vector, q.width) : 0;
   const uint64_t first = static_cast<uint64_t>(piece) * q.piece;
   const uint32_t last = q.tokens - first < q.piece ? q.tokens - 1 : static_cast<uint32_t>(first) + q.piece - 1;
   for (int side = 0; side < 2; side++) {
@@ -578,12 +640,34 @@ __device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float*
     uint32_t i = b > first ? b : static_cast<uint32_t>(first);
     const uint32_t end = e <= last ? e : last + 1;
     float acc[N] = {};
-    for (; i + 8 <= end; i += 8) {
-      Vec<T> v[8];
-      for (int k = 0; k < 8; k++) v[k] = Access<T>::load(values + q.by.order[i + k] * q.stride + column, q.width);
-      for (int k = 0; k < 8; k++) add<T>(acc, v[k]);
+    auto add_rows = [&](auto rows, auto order) {
+      constexpr int U = decltype(rows)::value;
+      Vec<T> v[U];
+#pragma unroll
+      for (int k = 0; k < U; k++) {
+        const uint32_t from = order(k);
+        if (mine) v[k] = Access<T>::load(values + from * q.stride + column, q.width);
+      }
+#pragma unroll
+      for (int k = 0; k < U; k++)
+        if (mine) add<T>(acc, v[k]);
+    };
+    if (WIDE) {
+      for (; i < end; i += 64) {
+        const uint32_t left = end - i < 64 ? end - i : 64, lane = threadIdx.x % 64;
+        const uint32_t order = lane < left ? q.by.order[i + lane] : 0;
+        uint32_t p = 0;
+        auto at = [&](int k) { return broadcast(order, p + k); };
+        for (; p + 16 <= left; p += 16) add_rows(std::integral_constant<int, 16>(), at);
+        if (p + 8 <= left) { add_rows(std::integral_constant<int, 8>(), at); p += 8; }
+        for (; p < left; p++) add_rows(std::integral_constant<int, 1>(), at);
+      }
+    } else {
+      auto at = [&](int k) { return q.by.order[i + k]; };
+      for (; i + 8 <= end; i += 8) add_rows(std::integral_constant<int, 8>(), at);
+      for (; i < end; i++) add_rows(std::integral_constant<int, 1>(), at);
     }
-    for (; i < end; i++) add<T>(acc, Access<T>::load(values + q.by.order[i] * q.stride + column, q.width));
+    if (!mine) continue;
     float* to = parts + (static_cast<uint64_t>(piece) * 2 + side) * q.parts_stride + column;
     const uint32_t skip = vector * N - column;   // what the vector before stores
     for (int n = 0; n < N; n++)
@@ -591,19 +675,24 @@ __device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float*
   }
 }
 
-template <typename T, bool NUMBERED>
+// WIDE: a row takes whole waves, so that all lanes of a wave have the same row.
+template <typename T, bool NUMBERED, bool WIDE>
 __global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float* parts, T* out) {
   __shared__ uint32_t empty[kZeroRows];
   if (blockIdx.x < q.piece_groups + q.window_groups) {
     const bool pieces = blockIdx.x < q.piece_groups;
     const uint32_t group = pieces ? blockIdx.x : blockIdx.x - q.piece_groups;
-    const uint32_t slot = threadIdx.x / q.lanes, vector = group % q.chunks * q.lanes + threadIdx.x % q.lanes;
-    if (slot >= q.rows_per_group || vector * Vec<T>::kCount >= q.width) return;
+    uint32_t slot = threadIdx.x / q.lanes;
+    if (WIDE) slot = broadcast(slot, 0);
+    const uint32_t vector = group % q.chunks * q.lanes + threadIdx.x % q.lanes;
+    const bool mine = vector * Vec<T>::kCount < q.width;
+    if (slot >= q.rows_per_group || (!WIDE && !mine)) return;
     const uint32_t number = group / q.chunks * q.rows_per_group + slot;
     if (pieces) {
-      if (number < q.pieces) sum_piece<T, NUMBERED>(q, values, parts, number, vector);
+      if (number < q.pieces) sum_piece<T, NUMBERED, WIDE>(q, values, parts, number, vector, mine);
     } else if (static_cast<uint64_t>(number) * kWindow < q.tokens) {
-      sum_window<T>(q, values, out, number, vector);
+      if (WIDE) sum_window_wide<T>(q, values, out, number, vector, mine);
+      else sum_window<T>(q, values, out, number, vector);
     }
     return;
   }
@@ -757,8 +846,10 @@ void sum_rows(const Layout& l, char* ws, const Sorted& by, const void* values, u
   q.piece_groups = groups(l.pieces);
   q.window_groups = groups((tokens + kWindow - 1) / kWindow);
   const uint32_t clearing = NUMBERED ? 0 : (rows + kZeroRows - 1) / kZeroRows;
-  hipLaunchKernelGGL((sum_kernel<T, NUMBERED>), dim3(q.piece_groups + q.window_groups + clearing), dim3(256), 0, stream, q,
-                     static_cast<const T*>(values), parts, static_cast<T*>(out));
+  const dim3 grid(q.piece_groups + q.window_groups + clearing);
+  const T* from = static_cast<const T*>(values);
+  if (s.lanes % 64 == 0) hipLaunchKernelGGL((sum_kernel<T, NUMBERED, true>), grid, dim3(256), 0, stream, q, from, parts, static_cast<T*>(out));
+  else hipLaunchKernelGGL((sum_kernel<T, NUMBERED, false>), grid, dim3(256), 0, stream, q, from, parts, static_cast<T*>(out));
   if (l.pieces)
     hipLaunchKernelGGL((join_kernel<T, NUMBERED>), dim3(q.piece_groups), dim3(256), 0, stream, q,
                        static_cast<const float*>(parts), static_cast<T*>(out));

@@ -215,7 +215,10 @@ int main(int argc, char** argv) {
     }
   }
   run({130, 40, 2100, 2100, STEP_BF16, STEP_I64, 2}, seed++);   // a row wider than a workgroup
-  run({200, 3, 300, 301, STEP_F32, STEP_I32, 1}, seed++);
+  run({200, 3, 300, 301, STEP_F32, STEP_I32, 1}, seed++);       // whole waves to a row, long runs
+  for (int kind = 0; kind < 6; kind++) run({300, 40, 131, 135, types[kind % 3], STEP_I64, kind}, seed++);
+  run({500, 12, 264, 264, STEP_BF16, STEP_I32, 0}, seed++);
+  run({130, 2, 257, 260, STEP_BF16, STEP_I64, 0}, seed++);
   run({5, 0, 4, 4, STEP_F32, STEP_I64, 4}, seed++);             // an empty table
   run({5, 9, 0, 0, STEP_F32, STEP_I64, 0}, seed++);             // no columns
   printf("step emulation: ok (%d cases)\n", g_cases);
