@@ -90,11 +90,12 @@ template <typename T> struct Access {
     }
     return v;
   }
-  // vector `vector` of the row that begins at `row`
-  static __device__ __forceinline__ void store(T* row, Vec<T> v, uint32_t vector, uint32_t width) {
+  // Vector `vector` of the row that begins at `row`. `passing`: see leaves_caches().
+  static __device__ __forceinline__ void store(T* row, Vec<T> v, uint32_t vector, uint32_t width, bool passing) {
     T* p = row + column(vector, width);
     if (vector * kCount + kCount <= width) {
-      *reinterpret_cast<RawU*>(p) = __builtin_bit_cast(Raw, v);
+      if (passing) __builtin_nontemporal_store(__builtin_bit_cast(Raw, v), reinterpret_cast<RawU*>(p));
+      else *reinterpret_cast<RawU*>(p) = __builtin_bit_cast(Raw, v);
     } else {
       const uint32_t skip = vector * kCount - column(vector, width);
       for (uint32_t k = 0; k < kCount; k++)
@@ -103,12 +104,18 @@ template <typename T> struct Access {
   }
 };
 
+// Whether a result is larger than the caches (256 MiB behind the L2s), so that no reader finds it there: its stores then
+// pass them by, and what is still to be read stays. A lookup of 131072 x 4096 bf16 rows 332 us without, 311 with; the
+// gradient of 100000 such rows from 65536 tokens 343 and 329 alone, 776 and 752 with an optimizer that reads it. Smaller
+// results lose: the gradient of 32000 such rows 100 and 93 alone, but 235 and 241 with its reader.
+bool leaves_caches(size_t rows, size_t width, size_t bytes) { return rows * width * bytes > size_t(256) << 20; }
+
 constexpr int kLookupRows = 4;  // rows a lane loads before it stores the first
 
 template <typename T>
 __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, const T* weight, uint32_t rows,
                               uint32_t width, uint64_t weight_stride, float scale, T* out, uint32_t lanes,
-                              uint32_t rows_per_group) {
+                              uint32_t rows_per_group, bool passing) {
   constexpr int N = Vec<T>::kCount;
   const uint32_t slot = threadIdx.x / lanes;
   const uint32_t vector = blockIdx.y * lanes + threadIdx.x % lanes;
@@ -128,7 +135,7 @@ __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, con
     if (t >= tokens) return;
     for (int e = 0; e < N; e++)
       v[k].at[e] = from_float<T>(key[k] < rows ? scale * to_float(v[k].at[e]) : 0.f);
-    Access<T>::store(out + t * width, v[k], vector, width);
+    Access<T>::store(out + t * width, v[k], vector, width, passing);
   }
 }
 
@@ -504,6 +511,7 @@ struct Sums {
   uint64_t stride, parts_stride;
   uint32_t tokens, rows, width;
   float scale;
+  bool passing;                             // leaves_caches()
   Sorted by;
   uint32_t piece, pieces;                   // length of a long run's parts, and how many places of that length there are
   uint32_t lanes, rows_per_group, chunks;   // RowShape
@@ -515,10 +523,11 @@ template <typename T> __device__ __forceinline__ void add(float (&acc)[Vec<T>::k
 }
 
 template <typename T>
-__device__ __forceinline__ void put(T* row, const float (&acc)[Vec<T>::kCount], float scale, uint32_t vector, uint32_t width) {
+__device__ __forceinline__ void put(T* row, const float (&acc)[Vec<T>::kCount], float scale, uint32_t vector, uint32_t width,
+                                    bool passing) {
   Vec<T> v;
   for (int n = 0; n < Vec<T>::kCount; n++) v.at[n] = from_float<T>(scale * acc[n]);
-  Access<T>::store(row, v, vector, width);
+  Access<T>::store(row, v, vector, width, passing);
 }
 
 // The runs that begin in a window and are no longer than a piece. A run's rows are added in the order of the tokens.
@@ -559,7 +568,7 @@ __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* ou
     for (int k = 0; k < 8; k++) {
       if (!take[k]) continue;
       if (begin[k]) {
-        if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+        if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
         open = row[k];
         for (int n = 0; n < N; n++) acc[n] = 0.f;
       }
@@ -567,7 +576,7 @@ __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* ou
     }
     if (stop || (open == kNoRow && i + 8 >= w1)) break;
   }
-  if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+  if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
 }
 
 // The same where a row takes whole waves: the lanes of a wave look at 64 places at once and hand what they saw to all.
@@ -580,7 +589,7 @@ __device__ __forceinline__ void sum_window_wide(const Sums& q, const T* values, 
   float acc[N];
   uint32_t open = kNoRow;
   auto close = [&]() {
-    if (mine && open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
+    if (mine && open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
   };
   for (uint64_t base = w0;; base += 64) {
     const uint64_t i = base + lane;
@@ -715,7 +724,7 @@ __global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float
   const uint32_t per_row = vectors < 64 ? vectors : (vectors + 63) / 64 * 64;
   for (uint32_t at = threadIdx.x; at < kZeroRows * static_cast<uint64_t>(per_row); at += 256) {
     const uint32_t k = at / per_row, vector = at % per_row;
-    if (vector < vectors && empty[k]) put<T>(out + (first + k) * q.width, zero, 1.f, vector, q.width);
+    if (vector < vectors && empty[k]) put<T>(out + (first + k) * q.width, zero, 1.f, vector, q.width, q.passing);
   }
 }
 
@@ -745,7 +754,7 @@ __global__ void __launch_bounds__(256) join_kernel(Sums q, const float* parts, T
   }
   for (; j < end; j++)
     for (int n = 0; n < N; n++) acc[n] += part(j)[n];
-  put<T>(out + static_cast<uint64_t>(run) * q.width, acc, q.scale, vector, q.width);
+  put<T>(out + static_cast<uint64_t>(run) * q.width, acc, q.scale, vector, q.width, q.passing);
 }
 
 // ---- host side --------------------------------------------------------------------
@@ -842,7 +851,8 @@ void sum_rows(const Layout& l, char* ws, const Sorted& by, const void* values, u
   const RowShape s = row_shape((width + Vec<T>::kCount - 1) / Vec<T>::kCount);
   float* parts = reinterpret_cast<float*>(ws + l.parts);
   auto groups = [&](uint64_t number) { return static_cast<uint32_t>((number + s.rows_per_group - 1) / s.rows_per_group * s.chunks); };
-  Sums q = {stride, l.parts_stride, tokens, rows, width, scale, by, l.piece, l.pieces, s.lanes, s.rows_per_group, s.chunks, 0, 0};
+  Sums q = {stride, l.parts_stride, tokens, rows, width, scale, leaves_caches(NUMBERED && tokens < rows ? tokens : rows, width, sizeof(T)),
+            by, l.piece, l.pieces, s.lanes, s.rows_per_group, s.chunks, 0, 0};
   q.piece_groups = groups(l.pieces);
   q.window_groups = groups((tokens + kWindow - 1) / kWindow);
   const uint32_t clearing = NUMBERED ? 0 : (rows + kZeroRows - 1) / kZeroRows;
@@ -860,6 +870,14 @@ __global__ void zero_kernel(uint32_t* to, uint64_t words, uint16_t* tail, int ha
   const uint64_t first = static_cast<uint64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
   for (uint64_t i = first; i < words; i += step) to[i] = 0;
   if (has_tail && first == 0) *tail = 0;
+}
+
+// Whether the largest launch of sum_rows stays under the 2^32 lanes of one (a lookup looks for itself).
+bool fits_launch(size_t tokens, size_t rows, size_t width, int dtype) {
+  const RowShape s = row_shape((width * dtype_size(dtype) + 15) / 16);
+  const uint64_t windows = (tokens + kWindow - 1) / kWindow, pieces = tokens / piece_for(tokens) + 1;
+  const uint64_t groups = (pieces / s.rows_per_group + windows / s.rows_per_group + 2) * s.chunks + rows / kZeroRows + 1;
+  return groups * 256 < uint64_t(1) << 32;
 }
 
 // A row's column ranges are grid y: 65535 of 256 lanes.
@@ -898,7 +916,7 @@ const char* step_status_string(int status) {
     case STEP_ERR_DTYPE: return "Invalid tensor type passed.";
     case STEP_ERR_ARGUMENT: return "invalid argument";
     case STEP_ERR_HIP: return "HIP runtime call failed";
-    case STEP_ERR_LIMIT: return "more than 2^31 - 1 tokens or rows, or 67107840 columns";
+    case STEP_ERR_LIMIT: return "more than 2^31 - 1 tokens or rows, 67107840 columns, or 2^32 - 1 lanes of a launch";
     default: return "unknown status";
   }
 }
@@ -913,13 +931,14 @@ int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const voi
   if (!out) return STEP_ERR_ARGUMENT;
   const RowShape s = row_shape((width * dtype_size(dtype) + 15) / 16);
   const size_t per_group = static_cast<size_t>(s.rows_per_group) * kLookupRows;
+  if ((tokens + per_group - 1) / per_group * 256 >= size_t(1) << 32) return STEP_ERR_LIMIT;  // lanes of a launch
   const dim3 grid(static_cast<uint32_t>((tokens + per_group - 1) / per_group), s.chunks);
   auto go = [&](auto type) {
     typedef decltype(type) T;
     hipLaunchKernelGGL((lookup_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), ids, id_type,
                        static_cast<uint32_t>(tokens), static_cast<const T*>(weight), static_cast<uint32_t>(rows),
                        static_cast<uint32_t>(width), static_cast<uint64_t>(weight_stride), scale, static_cast<T*>(out),
-                       s.lanes, s.rows_per_group);
+                       s.lanes, s.rows_per_group, leaves_caches(tokens, width, sizeof(T)));
   };
   if (dtype == STEP_F32) go(F32());
   else if (dtype == STEP_BF16) go(BF16());
@@ -950,6 +969,7 @@ int step_embedding_gradient(const void* ids, int id_type, size_t tokens, const v
                        reinterpret_cast<uint16_t*>(static_cast<char*>(out) + words * 4), bytes % 4 ? 1 : 0);
     return launched();
   }
+  if (!fits_launch(tokens, rows, width, dtype)) return STEP_ERR_LIMIT;
   const Layout l = layout_for(tokens, rows, width, false);
   if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
@@ -979,6 +999,7 @@ int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* val
     return launched();
   }
   if (!out_ids || (width && !out_values)) return STEP_ERR_ARGUMENT;
+  if (width && !fits_launch(tokens, 0, width, dtype)) return STEP_ERR_LIMIT;
   const Layout l = layout_for(tokens, rows, width, true);
   if (!workspace || workspace_bytes < l.bytes || reinterpret_cast<uintptr_t>(workspace) % 256) return STEP_ERR_ARGUMENT;
   char* ws = static_cast<char*>(workspace);
