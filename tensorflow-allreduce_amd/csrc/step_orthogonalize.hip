@@ -1126,6 +1126,8 @@ int run_round(const step_matrix* list, const Item* items, int count, int dtype, 
   return launched();
 }
 
+constexpr uint32_t kMostGrid = 1u << 22;  // workgroups of a launch, whose lanes have to stay below 2^32
+
 // A list of small matrices, those of up to 64 x 128 apart: two workgroups of them fit a compute unit's LDS.
 int run_small(const step_matrix* list, size_t length, int dtype, int out_dtype, const Rule& rule, hipStream_t stream) {
   bool any = false;
@@ -1154,9 +1156,15 @@ int run_small(const step_matrix* list, size_t length, int dtype, int out_dtype, 
     for (size_t k = 0; k < length; k++) {
       const step_matrix& x = list[k];
       if (x.rows == 0 || x.cols == 0 || x.count == 0 || (std::max(x.rows, x.cols) <= 128) != (across == 128)) continue;
-      if (items.count == kMostItems || x.count > kMostSize - matrices) flush();
-      items.at[items.count++] = {x.grad, x.momentum, x.out, matrices, static_cast<uint16_t>(x.rows), static_cast<uint16_t>(x.cols), x.rate};
-      matrices += static_cast<uint32_t>(x.count);
+      for (size_t first = 0, take; first < x.count; first += take) {
+        if (items.count == kMostItems || matrices == kMostGrid) flush();
+        take = std::min<size_t>(x.count - first, kMostGrid - matrices);
+        const size_t skip = first * x.rows * x.cols;
+        items.at[items.count++] = {static_cast<const char*>(x.grad) + skip * dtype_size(dtype), x.momentum ? x.momentum + skip : nullptr,
+                                   static_cast<char*>(x.out) + skip * dtype_size(out_dtype), matrices,
+                                   static_cast<uint16_t>(x.rows), static_cast<uint16_t>(x.cols), x.rate};
+        matrices += static_cast<uint32_t>(take);
+      }
     }
     flush();
   }

@@ -47,6 +47,7 @@ from . import _plugin, mpi_ops, ring_abi
 from ._plugin import (FailedPreconditionError, InternalError, InvalidArgumentError,  # noqa: F401
                       NotFoundError, OpError, UnknownError)
 from .mpi_ops import _allreduce, allgather, init, local_rank, rank, size  # noqa: F401
+from .step_ops import can_sum_slices as _can_sum_slices
 from .step_ops import (IndexedSlices, Muon, embedding, embedding_gradient, orthogonalize,  # noqa: F401
                        sum_slices)
 
@@ -811,6 +812,10 @@ class DistributedOptimizer:
         for g, p in grads_and_vars:
             g = _resolve(g.resolve() if isinstance(g, _FusedGrad) else g)
             if isinstance(g, IndexedSlices):
+                if not _can_sum_slices(g):
+                    idx = g.indices.reshape(1, -1)
+                    p.grad = torch.sparse_coo_tensor(idx, g.values, size=tuple(g.dense_shape)).coalesce()
+                    continue
                 # every rank's rows, one behind the other: one row for each index, the ranks' rows added in order
                 total = sum_slices(g)
                 p.grad = torch.sparse_coo_tensor(total.indices.long().reshape(1, -1), total.values,

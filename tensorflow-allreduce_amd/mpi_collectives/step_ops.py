@@ -99,7 +99,8 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
         scale: as in `embedding`.
 
     Sums are taken in 32 bits in the order of the tokens and rounded once to
-    grad's type; the same call gives the same bits every time."""
+    grad's type; the same call gives the same bits every time. The result is
+    differentiable with respect to grad."""
     what = "embedding_gradient"
     _check_tensor(grad, "grad", _FLOATS, what)
     _check_tensor(ids, "ids", _IDS, what)
@@ -109,6 +110,8 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
         _refuse("%s: rows is %d", what, rows)
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         _refuse("%s: a gradient of shape %s for ids of shape %s", what, tuple(grad.shape), tuple(ids.shape))
+    if grad.requires_grad and torch.is_grad_enabled():
+        return _EmbeddingGradient.apply(grad, ids, rows, float(scale))
     return _gradient(grad, ids, rows, float(scale))
 
 
@@ -135,6 +138,12 @@ def _gradient(grad, ids, rows, scale):
     return out
 
 
+def can_sum_slices(slices):
+    """Whether sum_slices takes the tensors of `slices`: their types, on a GPU."""
+    return (slices.values.is_cuda and slices.values.dtype in _FLOATS and slices.indices.is_cuda and
+            slices.indices.dtype in _IDS and slices.indices.dim() == 1)
+
+
 def sum_slices(slices):
     """An IndexedSlices with one row for each distinct index, in ascending order:
     the sum of the rows of `slices` that have it. This is what makes a gradient
@@ -149,7 +158,7 @@ def sum_slices(slices):
     Sums are taken in 32 bits in the order of the rows and rounded once; the
     same call gives the same bits every time. The number of distinct indices is
     read from the GPU, so the call waits for its stream and cannot be captured
-    into a graph."""
+    into a graph. No gradient flows through it."""
     what = "sum_slices"
     if not isinstance(slices, IndexedSlices):
         _refuse("%s: an IndexedSlices is needed, got %s", what, type(slices).__name__)
@@ -248,7 +257,8 @@ def embedding(ids, weight, scale=1.0, sparse=False):
                 it is a sparse tensor with one row per distinct id, which
                 DistributedOptimizer exchanges as an IndexedSlices; its size
                 depends on the data, so that backward pass waits for its stream
-                and cannot be captured into a graph.
+                and cannot be captured into a graph. Where gradients of
+                gradients are asked for (create_graph) it is dense all the same.
     """
     what = "embedding"
     _check_tensor(ids, "ids", _IDS, what)
@@ -299,7 +309,8 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
                 about 1e-6 off. Default: True if the result is float32. Matrices
                 of at most 64 x 256 (or the transposed) are always precise.
 
-    An update with an infinity or NaN gives NaN."""
+    An update with an infinity or NaN gives NaN. No gradient flows through the
+    result."""
     what = "orthogonalize"
     _check_tensor(update, "update", _FLOATS, what)
     if update.dim() < 2:
@@ -332,6 +343,9 @@ class Muon(torch.optim.Optimizer):
         M <- momentum M + G
         U  = G + momentum M  (nesterov)  or  M
         W <- W (1 - lr weight_decay) - lr s orthogonalize(U)
+
+    A step can be captured into a graph once every momentum exists, that is after
+    a step of its own; lr and the other options are then those of the capture.
 
     Made to be wrapped by DistributedOptimizer. All matrices of a step go through
     each product in one launch. Embeddings, biases and other vectors belong to
@@ -402,6 +416,9 @@ class Muon(torch.optim.Optimizer):
             state = self.state[p]
             m = state.get("momentum_buffer")
             if m is None:
+                if torch.cuda.is_current_stream_capturing():
+                    _refuse("Muon: a first step cannot be captured into a graph, whose replays would begin with a momentum "
+                            "of zero again; take one before")
                 m = state["momentum_buffer"] = torch.zeros(p.shape, dtype=torch.float32, device=device)
             elif m.dtype != torch.float32 or m.device != device or m.shape != p.shape or not m.is_contiguous():
                 _refuse("Muon: a momentum buffer of shape %s and type %s on %s", tuple(m.shape), m.dtype, m.device)
@@ -427,6 +444,7 @@ class Muon(torch.optim.Optimizer):
             ws.data_ptr(), size, _stream_of(device.index)), "Muon.step")
         for p, w in moved:
             p.copy_(w)
+        torch.autograd.graph.increment_version(params)  # a backward pass that still needs the old weights has to notice
 
     def load_state_dict(self, state_dict):
         """Unlike the base class, which gives every buffer its parameter's type, this keeps the momentum in float32."""

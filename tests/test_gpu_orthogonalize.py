@@ -347,3 +347,74 @@ def test_a_training_step_through_the_exchange(fusion):
     for p, want in zip(nets[0], mirror):
         # float32 gradients are some 2^-20 off, and a step turns and stretches them by at most 485 (a^5); three steps
         assert distance(p, want.detach()) <= 3 * 485 * 2.0 ** -20
+
+
+def test_muon_tells_autograd_and_refuses_a_captured_first_step():
+    w = torch.nn.Parameter(gradient(30, 70, 90))
+    opt = mpi.Muon([w])
+    loss = (w * w).sum()                    # its backward pass needs the weights as they are now
+    w.grad = gradient(31, 70, 90)
+    opt.step()
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    v = torch.nn.Parameter(w.detach().clone())
+    v.grad = gradient(32, 70, 90)
+    before = v.detach().clone()
+    opt = mpi.Muon([v])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side), torch.cuda.graph(g, stream=side):
+        with pytest.raises(mpi.InvalidArgumentError):
+            opt.step()
+    torch.cuda.synchronize()
+    assert torch.equal(v, before) and not opt.state[v]
+
+
+@pytest.mark.parametrize("shape", [(140_000, 64, 256), (1100, 2048, 1024)])
+def test_batches_beyond_32_bits(shape):
+    """More than 2^31 elements and 2^32 bytes: the last matrix comes out as it does alone."""
+    one = gradient(40, *shape[1:], dtype=torch.bfloat16)
+    batch = torch.zeros(shape, dtype=torch.bfloat16, device="cuda")
+    batch[-1] = one
+    batch[0] = one
+    got = mpi.orthogonalize(batch)
+    want = mpi.orthogonalize(one)
+    assert distance(want, exact(one)) <= bound(torch.bfloat16, False, shape)
+    tolerance = 2 * bound(torch.bfloat16, False, shape)   # a list of another size may take other tiles, in another order
+    assert distance(got[-1], want) <= tolerance and distance(got[0], want) <= tolerance
+    assert not bool(got[1].any()) and not bool(got[-2].any())
+
+
+def test_more_matrices_than_workgroups_of_a_launch():
+    """2^32 lanes are 8388608 workgroups of 512: a batch of more is several launches."""
+    count = (1 << 23) + 5
+    batch = torch.ones(count, 1, 2, device="cuda")
+    batch[:, 0, 1] = torch.arange(count, device="cuda") % 7
+    got = mpi.orthogonalize(batch, steps=2)
+    want = mpi.orthogonalize(batch[:7], steps=2)
+    assert torch.equal(got[:7 * 1000].view(1000, 7, 1, 2), want.expand(1000, 7, 1, 2))
+    last = torch.arange(count - 7, count, device="cuda") % 7
+    assert torch.equal(got[-7:], want[last])
+    middle = torch.arange((1 << 22) - 7, (1 << 22) + 7, device="cuda")
+    assert torch.equal(got[middle], want[middle % 7])
+
+
+def test_a_matrix_beyond_32_bits():
+    """One matrix of more than 2^31 elements, a single step; its ends against X a + X (b A + c A A). That X is the rounded
+    update over its norm; all of it is a sum of about 2100 products of which X's own rounding is the largest."""
+    rows, cols = 1 << 20, 2100
+    update = torch.empty(rows, cols, dtype=torch.bfloat16, device="cuda")
+    for k in range(0, rows, 1 << 17):
+        update[k:k + (1 << 17)] = torch.randn(1 << 17, cols, generator=torch.Generator("cuda").manual_seed(k), device="cuda")
+    got = mpi.orthogonalize(update, steps=1)
+    gram, size = torch.zeros(cols, cols, dtype=torch.float64, device="cuda"), 0.0
+    for k in range(0, rows, 1 << 15):
+        part = update[k:k + (1 << 15)].float()
+        gram += (part.T.contiguous() @ part).double()
+        size += float(part.square().sum(dtype=torch.float64))
+    gram /= size
+    inner = B * gram + C * gram @ gram
+    for at in (slice(0, 300), slice(rows // 2, rows // 2 + 300), slice(rows - 300, rows)):
+        x = update[at].double() / math.sqrt(size)
+        assert distance(got[at], A * x + x @ inner) <= bound(torch.bfloat16, False, (rows, cols))

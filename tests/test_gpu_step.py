@@ -376,3 +376,14 @@ def test_gradient_of_the_gradient():
     want, = torch.autograd.grad((picked * mirror_m).sum(), mirror_w, create_graph=True)
     want.square().sum().backward()
     assert torch.allclose(mix.grad.double().cpu(), mirror_m.grad, rtol=40 * U, atol=40 * U * float(mirror_m.grad.abs().max()))
+
+
+def test_the_gradient_called_by_name_is_differentiable():
+    """embedding_gradient is linear in grad: the gradient of <embedding_gradient(g), m> is the lookup of m."""
+    ids = make_ids(70, 50, 9, "padded", torch.int32)
+    grad = values(71, 50, 12).requires_grad_(True)
+    mix = values(72, 9, 12)
+    (mpi.embedding_gradient(grad, ids, 9, scale=0.5) * mix).sum().backward()
+    assert torch.equal(grad.grad, mpi.embedding(ids, mix, scale=0.5))
+    with torch.no_grad():
+        assert not mpi.embedding_gradient(grad, ids, 9).requires_grad

@@ -98,6 +98,26 @@ def _assembly(source):
     return open(asm).read()
 
 
+def test_embedding_refuses_what_no_launch_holds():
+    """A launch has less than 2^32 lanes; the pointers are never followed."""
+    lib = step_abi.lib()
+    p, big = 4096, 1 << 62
+
+    def lookup(tokens, width):
+        return lib.step_embedding_lookup(p, 1, tokens, p, 3, 100, width, width, 1.0, p, None)
+
+    def gradient(tokens, rows, width):
+        return lib.step_embedding_gradient(p, 1, tokens, p, 3, rows, width, width, 1.0, p, p, big, None)
+
+    def slices(tokens, width):
+        return lib.step_sum_slices(p, 1, tokens, p, 3, 100, width, width, 1.0, p, p, p, p, big, None)
+
+    limit = 5
+    assert lookup(1 << 26, 2048) == lookup((1 << 31) - 1, 512) == limit
+    assert gradient(1 << 27, 100, 2048) == gradient(1 << 26, 100, 4096) == gradient(100, 1 << 30, 1) == limit
+    assert slices(1 << 27, 2048) == slices(1 << 26, 4096) == limit
+
+
 def test_orthogonalize_refuses_on_the_host():
     """The C entry points' own checks, with pointers that are never followed."""
     lib = step_abi.lib()
@@ -140,3 +160,12 @@ def test_embedding_assembly():
     assert not found, "scalar selects on a stale condition code: %r" % (found[:5],)
     kernels = kernels_in_scratch(text, ("lookup_kernel", "sort_one_kernel", "scatter_kernel", "sum_kernel", "join_kernel"))
     assert kernels["seen"] >= 17 and not kernels["scratch"], kernels
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])
+def test_slices_on_the_cpu_are_applied_as_ever(dtype):
+    """apply_gradients with slices that are not on the GPU, or of a type that sum_slices does not take."""
+    w = torch.zeros(5, 3, dtype=dtype, requires_grad=True)
+    slices = mpi.IndexedSlices(torch.ones(4, 3, dtype=dtype), torch.tensor([1, 4, 1, 0]), (5, 3))
+    mpi.DistributedOptimizer(torch.optim.SGD([w], lr=1.0)).apply_gradients([(slices, w)])
+    assert w[:, 0].tolist() == [-1.0, -2.0, 0.0, 0.0, -1.0] and w.grad.is_coalesced()
