@@ -90,11 +90,12 @@ template <typename T> struct Access {
     }
     return v;
   }
-  // Vector `vector` of the row that begins at `row`. `passing`: see leaves_caches().
-  static __device__ __forceinline__ void store(T* row, Vec<T> v, uint32_t vector, uint32_t width, bool passing) {
+  // Vector `vector` of the row that begins at `row`. PASSING: see leaves_caches(). (No argument: the compiler makes one
+  // unmarked store of the two sides of a branch.)
+  template <bool PASSING> static __device__ __forceinline__ void store(T* row, Vec<T> v, uint32_t vector, uint32_t width) {
     T* p = row + column(vector, width);
     if (vector * kCount + kCount <= width) {
-      if (passing) __builtin_nontemporal_store(__builtin_bit_cast(Raw, v), reinterpret_cast<RawU*>(p));
+      if (PASSING) __builtin_nontemporal_store(__builtin_bit_cast(Raw, v), reinterpret_cast<RawU*>(p));
       else *reinterpret_cast<RawU*>(p) = __builtin_bit_cast(Raw, v);
     } else {
       const uint32_t skip = vector * kCount - column(vector, width);
@@ -112,10 +113,10 @@ bool leaves_caches(size_t rows, size_t width, size_t bytes) { return rows * widt
 
 constexpr int kLookupRows = 4;  // rows a lane loads before it stores the first
 
-template <typename T>
+template <typename T, bool PASSING>
 __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, const T* weight, uint32_t rows,
                               uint32_t width, uint64_t weight_stride, float scale, T* out, uint32_t lanes,
-                              uint32_t rows_per_group, bool passing) {
+                              uint32_t rows_per_group) {
   constexpr int N = Vec<T>::kCount;
   const uint32_t slot = threadIdx.x / lanes;
   const uint32_t vector = blockIdx.y * lanes + threadIdx.x % lanes;
@@ -135,7 +136,7 @@ __global__ void lookup_kernel(const void* ids, int id_type, uint32_t tokens, con
     if (t >= tokens) return;
     for (int e = 0; e < N; e++)
       v[k].at[e] = from_float<T>(key[k] < rows ? scale * to_float(v[k].at[e]) : 0.f);
-    Access<T>::store(out + t * width, v[k], vector, width, passing);
+    Access<T>::template store<PASSING>(out + t * width, v[k], vector, width);
   }
 }
 
@@ -511,7 +512,6 @@ struct Sums {
   uint64_t stride, parts_stride;
   uint32_t tokens, rows, width;
   float scale;
-  bool passing;                             // leaves_caches()
   Sorted by;
   uint32_t piece, pieces;                   // length of a long run's parts, and how many places of that length there are
   uint32_t lanes, rows_per_group, chunks;   // RowShape
@@ -522,16 +522,15 @@ template <typename T> __device__ __forceinline__ void add(float (&acc)[Vec<T>::k
   for (int n = 0; n < Vec<T>::kCount; n++) acc[n] += to_float(v.at[n]);
 }
 
-template <typename T>
-__device__ __forceinline__ void put(T* row, const float (&acc)[Vec<T>::kCount], float scale, uint32_t vector, uint32_t width,
-                                    bool passing) {
+template <typename T, bool PASSING>
+__device__ __forceinline__ void put(T* row, const float (&acc)[Vec<T>::kCount], float scale, uint32_t vector, uint32_t width) {
   Vec<T> v;
   for (int n = 0; n < Vec<T>::kCount; n++) v.at[n] = from_float<T>(scale * acc[n]);
-  Access<T>::store(row, v, vector, width, passing);
+  Access<T>::template store<PASSING>(row, v, vector, width);
 }
 
 // The runs that begin in a window and are no longer than a piece. A run's rows are added in the order of the tokens.
-template <typename T>
+template <typename T, bool PASSING>
 __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* out, uint32_t window, uint32_t vector) {
   constexpr int N = Vec<T>::kCount;
   const uint32_t column = Access<T>::column(vector, q.width);
@@ -568,7 +567,7 @@ __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* ou
     for (int k = 0; k < 8; k++) {
       if (!take[k]) continue;
       if (begin[k]) {
-        if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
+        if (open != kNoRow) put<T, PASSING>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
         open = row[k];
         for (int n = 0; n < N; n++) acc[n] = 0.f;
       }
@@ -576,12 +575,12 @@ __device__ __forceinline__ void sum_window(const Sums& q, const T* values, T* ou
     }
     if (stop || (open == kNoRow && i + 8 >= w1)) break;
   }
-  if (open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
+  if (open != kNoRow) put<T, PASSING>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
 }
 
 // The same where a row takes whole waves: the lanes of a wave look at 64 places at once and hand what they saw to all.
 // `mine`: whether this lane has columns; the others only look.
-template <typename T>
+template <typename T, bool PASSING>
 __device__ __forceinline__ void sum_window_wide(const Sums& q, const T* values, T* out, uint32_t window, uint32_t vector, bool mine) {
   constexpr int N = Vec<T>::kCount;
   const uint32_t column = mine ? Access<T>::column(vector, q.width) : 0, lane = threadIdx.x % 64;
@@ -589,7 +588,7 @@ __device__ __forceinline__ void sum_window_wide(const Sums& q, const T* values, 
   float acc[N];
   uint32_t open = kNoRow;
   auto close = [&]() {
-    if (mine && open != kNoRow) put<T>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width, q.passing);
+    if (mine && open != kNoRow) put<T, PASSING>(out + static_cast<uint64_t>(open) * q.width, acc, q.scale, vector, q.width);
   };
   for (uint64_t base = w0;; base += 64) {
     const uint64_t i = base + lane;
@@ -685,7 +684,7 @@ __device__ __forceinline__ void sum_piece(const Sums& q, const T* values, float*
 }
 
 // WIDE: a row takes whole waves, so that all lanes of a wave have the same row.
-template <typename T, bool NUMBERED, bool WIDE>
+template <typename T, bool NUMBERED, bool WIDE, bool PASSING>
 __global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float* parts, T* out) {
   __shared__ uint32_t empty[kZeroRows];
   if (blockIdx.x < q.piece_groups + q.window_groups) {
@@ -700,8 +699,8 @@ __global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float
     if (pieces) {
       if (number < q.pieces) sum_piece<T, NUMBERED, WIDE>(q, values, parts, number, vector, mine);
     } else if (static_cast<uint64_t>(number) * kWindow < q.tokens) {
-      if (WIDE) sum_window_wide<T>(q, values, out, number, vector, mine);
-      else sum_window<T>(q, values, out, number, vector);
+      if (WIDE) sum_window_wide<T, PASSING>(q, values, out, number, vector, mine);
+      else sum_window<T, PASSING>(q, values, out, number, vector);
     }
     return;
   }
@@ -724,7 +723,7 @@ __global__ void __launch_bounds__(256) sum_kernel(Sums q, const T* values, float
   const uint32_t per_row = vectors < 64 ? vectors : (vectors + 63) / 64 * 64;
   for (uint32_t at = threadIdx.x; at < kZeroRows * static_cast<uint64_t>(per_row); at += 256) {
     const uint32_t k = at / per_row, vector = at % per_row;
-    if (vector < vectors && empty[k]) put<T>(out + (first + k) * q.width, zero, 1.f, vector, q.width, q.passing);
+    if (vector < vectors && empty[k]) put<T, PASSING>(out + (first + k) * q.width, zero, 1.f, vector, q.width);
   }
 }
 
@@ -754,7 +753,7 @@ __global__ void __launch_bounds__(256) join_kernel(Sums q, const float* parts, T
   }
   for (; j < end; j++)
     for (int n = 0; n < N; n++) acc[n] += part(j)[n];
-  put<T>(out + static_cast<uint64_t>(run) * q.width, acc, q.scale, vector, q.width, q.passing);
+  put<T, false>(out + static_cast<uint64_t>(run) * q.width, acc, q.scale, vector, q.width);
 }
 
 // ---- host side --------------------------------------------------------------------
@@ -851,15 +850,19 @@ void sum_rows(const Layout& l, char* ws, const Sorted& by, const void* values, u
   const RowShape s = row_shape((width + Vec<T>::kCount - 1) / Vec<T>::kCount);
   float* parts = reinterpret_cast<float*>(ws + l.parts);
   auto groups = [&](uint64_t number) { return static_cast<uint32_t>((number + s.rows_per_group - 1) / s.rows_per_group * s.chunks); };
-  Sums q = {stride, l.parts_stride, tokens, rows, width, scale, leaves_caches(NUMBERED && tokens < rows ? tokens : rows, width, sizeof(T)),
-            by, l.piece, l.pieces, s.lanes, s.rows_per_group, s.chunks, 0, 0};
+  Sums q = {stride, l.parts_stride, tokens, rows, width, scale, by, l.piece, l.pieces, s.lanes, s.rows_per_group, s.chunks, 0, 0};
   q.piece_groups = groups(l.pieces);
   q.window_groups = groups((tokens + kWindow - 1) / kWindow);
   const uint32_t clearing = NUMBERED ? 0 : (rows + kZeroRows - 1) / kZeroRows;
   const dim3 grid(q.piece_groups + q.window_groups + clearing);
   const T* from = static_cast<const T*>(values);
-  if (s.lanes % 64 == 0) hipLaunchKernelGGL((sum_kernel<T, NUMBERED, true>), grid, dim3(256), 0, stream, q, from, parts, static_cast<T*>(out));
-  else hipLaunchKernelGGL((sum_kernel<T, NUMBERED, false>), grid, dim3(256), 0, stream, q, from, parts, static_cast<T*>(out));
+  const bool passing = leaves_caches(NUMBERED && tokens < rows ? tokens : rows, width, sizeof(T));
+  auto go = [&](auto wide, auto pass) {
+    hipLaunchKernelGGL((sum_kernel<T, NUMBERED, decltype(wide)::value, decltype(pass)::value>), grid, dim3(256), 0, stream, q, from,
+                       parts, static_cast<T*>(out));
+  };
+  if (s.lanes % 64) passing ? go(std::false_type(), std::true_type()) : go(std::false_type(), std::false_type());
+  else passing ? go(std::true_type(), std::true_type()) : go(std::true_type(), std::false_type());
   if (l.pieces)
     hipLaunchKernelGGL((join_kernel<T, NUMBERED>), dim3(q.piece_groups), dim3(256), 0, stream, q,
                        static_cast<const float*>(parts), static_cast<T*>(out));
@@ -933,16 +936,20 @@ int step_embedding_lookup(const void* ids, int id_type, size_t tokens, const voi
   const size_t per_group = static_cast<size_t>(s.rows_per_group) * kLookupRows;
   if ((tokens + per_group - 1) / per_group * 256 >= size_t(1) << 32) return STEP_ERR_LIMIT;  // lanes of a launch
   const dim3 grid(static_cast<uint32_t>((tokens + per_group - 1) / per_group), s.chunks);
-  auto go = [&](auto type) {
+  auto go = [&](auto type, auto pass) {
     typedef decltype(type) T;
-    hipLaunchKernelGGL((lookup_kernel<T>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), ids, id_type,
+    hipLaunchKernelGGL((lookup_kernel<T, decltype(pass)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), ids, id_type,
                        static_cast<uint32_t>(tokens), static_cast<const T*>(weight), static_cast<uint32_t>(rows),
                        static_cast<uint32_t>(width), static_cast<uint64_t>(weight_stride), scale, static_cast<T*>(out),
-                       s.lanes, s.rows_per_group, leaves_caches(tokens, width, sizeof(T)));
+                       s.lanes, s.rows_per_group);
   };
-  if (dtype == STEP_F32) go(F32());
-  else if (dtype == STEP_BF16) go(BF16());
-  else go(F16());
+  auto by_size = [&](auto type) {
+    if (leaves_caches(tokens, width, dtype_size(dtype))) go(type, std::true_type());
+    else go(type, std::false_type());
+  };
+  if (dtype == STEP_F32) by_size(F32());
+  else if (dtype == STEP_BF16) by_size(BF16());
+  else by_size(F16());
   return launched();
 }
 
