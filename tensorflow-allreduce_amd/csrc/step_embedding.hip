@@ -154,7 +154,9 @@ constexpr int kBins = 1 << kMostDigitBits;
 constexpr uint32_t kSortThreads = STEP_SORT_THREADS;
 constexpr uint32_t kWaves = kSortThreads / 64;
 static_assert(kSortThreads >= static_cast<uint32_t>(kBins), "one lane per digit");
-constexpr uint32_t kOneGroup = 8 * kSortThreads;          // tokens one workgroup sorts in LDS
+// Tokens one workgroup sorts in LDS. Numbering the runs takes two launches more where several workgroups sort: 10007 tokens
+// of 64 columns as slices 65 us in one workgroup and 73 in several, as a gradient 39 either way (8192: 33 in one).
+constexpr uint32_t kOneGroup = 8 * kSortThreads, kOneGroupNumbered = 12 * kSortThreads;
 constexpr int kTileKeys = 4;                              // keys per lane of a tile of the several-workgroup sort
 constexpr uint32_t kTile = kSortThreads * kTileKeys;
 // above that many tiles each pass would spend its time reading counts; tiles get longer instead
@@ -265,7 +267,7 @@ struct Sorted {
 };
 
 // Everything of the sort in one workgroup's LDS, and the runs. Bound by the chain of ballots and LDS accesses of a round of
-// 64 keys per wave: 1024 tokens 7 us, 2048 11, 4096 15, 8192 23 (two passes). Above, several workgroups: 8193 tokens 32 us
+// 64 keys per wave: 1024 tokens 7 us, 2048 11, 4096 15, 8192 23, 12288 30 (two passes). Above, several workgroups: 8193 tokens 32 us
 // in five launches (count 3, scatter 11 per pass, runs 4), 65536 tokens 36.
 template <int K>
 __global__ void __launch_bounds__(kSortThreads) sort_one_kernel(const void* ids, int id_type, uint32_t tokens,
@@ -793,7 +795,7 @@ Layout layout_for(size_t tokens, size_t rows, size_t width, bool numbered) {
   if (tokens > static_cast<size_t>(kTile) * kMostTiles)
     l.tile_length = static_cast<uint32_t>(round_up((tokens + kMostTiles - 1) / kMostTiles, kTile));
   l.tiles = static_cast<uint32_t>((tokens + l.tile_length - 1) / l.tile_length);
-  const bool one = tokens <= kOneGroup;
+  const bool one = tokens <= (numbered ? kOneGroupNumbered : kOneGroup);
   for (int k = 0; k < 2; k++) {
     l.keys[k] = take(one ? (k ? 0 : tokens * 4) : tokens * 4);
     l.order[k] = take(one ? (k ? 0 : tokens * 4) : tokens * 4);
@@ -815,7 +817,7 @@ Sorted sort_tokens(const Layout& l, char* ws, const void* ids, int id_type, uint
   auto at = [ws](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
   const Digits d = digits_for(rows);
   Sorted to = {at(l.order[0]), at(l.row_of), at(l.begin), at(l.end)};
-  if (tokens <= kOneGroup) {
+  if (tokens <= (numbered ? kOneGroupNumbered : kOneGroup)) {
     auto sort = [&](auto keys) {
       hipLaunchKernelGGL((sort_one_kernel<decltype(keys)::value>), dim3(1), dim3(kSortThreads), 0, stream, ids, id_type,
                          tokens, rows, d.bits, d.passes, to, numbered ? 1 : 0, out_ids, out_count);
@@ -823,7 +825,8 @@ Sorted sort_tokens(const Layout& l, char* ws, const void* ids, int id_type, uint
     if (tokens <= kSortThreads) sort(std::integral_constant<int, 1>());
     else if (tokens <= 2 * kSortThreads) sort(std::integral_constant<int, 2>());
     else if (tokens <= 4 * kSortThreads) sort(std::integral_constant<int, 4>());
-    else sort(std::integral_constant<int, 8>());
+    else if (tokens <= 8 * kSortThreads) sort(std::integral_constant<int, 8>());
+    else sort(std::integral_constant<int, 12>());
     return to;
   }
   const uint32_t* keys = nullptr;

@@ -259,6 +259,10 @@ def embedding(ids, weight, scale=1.0, sparse=False):
                 depends on the data, so that backward pass waits for its stream
                 and cannot be captured into a graph. Where gradients of
                 gradients are asked for (create_graph) it is dense all the same.
+
+    A forward and backward pass can be captured into a graph. As with every
+    function of torch, no eager graph of the same leaves may be alive then:
+    autograd would join its stream into the capture.
     """
     what = "embedding"
     _check_tensor(ids, "ids", _IDS, what)

@@ -204,7 +204,7 @@ int main(int argc, char** argv) {
   refusals();
   unsigned seed = 1;
   const int types[3] = {STEP_F32, STEP_BF16, STEP_F16};
-  const size_t tokens[] = {0, 1, 2, 63, 64, 65, 127, 129, 300, 700, 1023, 1024, 1025, 1700};
+  const size_t tokens[] = {0, 1, 2, 63, 64, 65, 127, 129, 300, 700, 1023, 1024, 1025, 1700, 1536, 1537};
   const size_t widths[] = {1, 7, 8, 33, 65};
   for (size_t k = 0; k < sizeof(tokens) / sizeof(tokens[0]); k++) {
     for (int kind = 0; kind < 6; kind++) {

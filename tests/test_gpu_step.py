@@ -73,7 +73,7 @@ def assert_sums(got, total, size, count, scale, dtype):
 
 
 SHAPES = [(1, 1, 1), (1, 50, 8), (2, 7, 3), (63, 9, 64), (64, 1000, 65), (257, 33, 1001), (1000, 4000, 129),
-          (1024, 300, 256), (1025, 5000, 40), (5000, 777, 515), (8192, 8192, 16), (8193, 100, 24), (20001, 70000, 33)]
+          (1024, 300, 256), (1025, 5000, 40), (5000, 777, 515), (8192, 8192, 16), (8193, 100, 24), (12288, 9000, 20), (12289, 300, 20), (20001, 70000, 33)]
 
 
 @pytest.mark.parametrize("dtype", FLOATS)
@@ -173,7 +173,8 @@ def test_gradient_strides():
 
 @pytest.mark.parametrize("tokens, ranks, rows, width, id_type", [
     (1, 1, 10, 5, torch.int64), (0, 3, 10, 5, torch.int32), (129, 4, 3000, 300, torch.int64), (700, 3, 90, 33, torch.int32),
-    (3000, 8, 5021, 64, torch.int64), (5000, 16, 12, 9, torch.int32)])
+    (3000, 8, 5021, 64, torch.int64), (5000, 16, 12, 9, torch.int32),
+    (1536, 8, 400, 20, torch.int64)])
 def test_sum_slices(tokens, ranks, rows, width, id_type):
     ids = torch.cat([make_ids(20 + r, tokens, rows, "common" if r % 2 else "padded", id_type) for r in range(ranks)])
     grad = values(11, tokens * ranks, width)
