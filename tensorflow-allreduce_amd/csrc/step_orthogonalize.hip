@@ -17,7 +17,9 @@
 // is kept: X = hi + lo / 2048 in two fp16 planes, and the linear term a X counts
 // both. Without that, rounding noise in the directions that U hardly has grows by
 // a factor of a = 3.4 per step (485 in five), until it is 14 % of the result for
-// an update of rank one, and with it 0.03 to 0.2 % whatever the rank.
+// an update of rank one, and with it 0.05 to 0.3 % whatever the rank (norm of the
+// difference over that of the result; up to 0.6 % where an update has fewer than
+// eight rows, whose few roundings hit everything).
 //   SPLIT = false (16-bit results): products of the hi planes.
 //   (The last iterate but one does without: its rounding grows by a once.)
 //   SPLIT = true (float32 results): hi hi + (hi lo + lo hi) / 2048, three products,
@@ -59,7 +61,7 @@ constexpr int kMostSteps = 64;
 // ---- where a matrix keeps its planes -------------------------------------------
 
 struct Planes {
-  uint64_t norm, x_hi, x_lo, y_hi, y_lo, a_hi, a_lo, b_hi, b_lo, bytes;
+  uint64_t norm, x_hi, x_lo, y_hi, y_lo, a_hi, a_lo, b_hi, b_lo, b_rest, bytes;
   uint64_t y_hi_step, y_lo_step;  // Y has two buffers that take turns; its low plane needs one only if no product reads it
 };
 
@@ -83,6 +85,8 @@ __host__ __device__ inline Planes planes_of(uint64_t m, uint64_t n, bool split) 
     p.x_lo = at; at += mn;
     p.a_lo = at; at += mm;
     p.b_lo = at; at += mm;
+  } else {
+    p.b_rest = at; at += m * 2;  // what B's diagonal lost when it was rounded
   }
   p.bytes = round_up(at, 256);
   return p;
@@ -291,7 +295,11 @@ __global__ void __launch_bounds__(256) first_kernel(Segments segments, MomentumR
 // ---- products -----------------------------------------------------------------------
 
 // A = X X^T; B = a I + b A + c A A; the next X = B X and its Y; the last X, to the caller. The linear term is on B's
-// diagonal, so that the products add it: no pass reads X for it, but the low plane where they do not.
+// diagonal, so that the products add it: no pass reads X for it, but the low plane where they do not. In fp16 that
+// diagonal, 1024 * 3.4 and more, is off by up to 2^-12 of itself, which every later step stretches: where there is no low
+// plane of B, what was rounded off its diagonal is kept apart (b_rest) and multiplied as a diagonal matrix, one more product
+// of 16 x 16 x 32 for each of a wave's pieces. Without it, updates of rank one are 0.24 % off at any size (2-norm); with it
+// 0.06 % at 128 rows and 0.02 % at 1000.
 enum Kind { GRAM, SQUARE, APPLY, LAST };
 
 // Moves 16 bytes per lane from global memory into LDS at base + 16 * lane, without registers in between.
@@ -495,6 +503,49 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
         }
       }
   };
+  // What B's diagonal lost, as diagonal matrices of 32 rows (a pair of pieces), times those rows of X. Tiles of up to 128 take
+  // them from LDS while their stage is there; of 256 once more from the L2 behind the last one, as a branch in the main loop
+  // costs them their registers. (B X of 16 1024 x 1024: 53.1 us without, 58.4 all
+  // from the L2, 56.4 from LDS.)
+  constexpr bool REST = FROM_Y && !SPLIT, FROM_LDS = SIDE < 256;
+  static_assert(!REST || PAIR_P, "");
+  const uint32_t rest_row = lane % 16 / 4 * 8 + lane % 4;
+  _Float16 rest[REST ? FM : 1];
+  auto fetch_rest = [&]() {
+    if constexpr (REST) {
+#pragma unroll
+      for (int x = 0; x < FM; x++) {
+        const uint32_t row = i0 + wi + x / 2 * 32 + x % 2 * 4 + rest_row;
+        rest[x] = reinterpret_cast<const _Float16*>(at + p.b_rest)[row < m ? row : m - 1];
+      }
+    }
+  };
+  auto add_rest = [&](int x, int y, half8 q) {
+    half8 d0 = {}, d1 = {};
+#pragma unroll
+    for (uint32_t e = 0; e < 4; e++) {
+      const bool here = lane / 16 == lane % 16 / 4 && lane % 4 == e;
+      d0[e] = here ? rest[x] : static_cast<_Float16>(0);
+      d1[e + 4] = here ? rest[x + 1] : static_cast<_Float16>(0);
+    }
+    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d0, q, acc[x][y], 0, 0, 0);
+    acc[x + 1][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d1, q, acc[x + 1][y], 0, 0, 0);
+  };
+  auto add_rest_of = [&](uint32_t stage, uint32_t buffer) {
+    if constexpr (REST && FROM_LDS) {
+#pragma unroll
+      for (int x = 0; x < FM; x += 2) {
+        const uint32_t half = (i0 + wi) / 32 + x / 2, chunk = half % 2 * 4 + lane / 16;
+        if (half / 2 != stage) continue;
+#pragma unroll
+        for (int y = 0; y < FN; y++) {
+          const uint32_t row = wj + row_of_piece<PAIR_Q>(y, lane % 16);
+          add_rest(x, y, *reinterpret_cast<const half8*>(lds + (buffer * KS + mine) * SUB + (SIDE + row) * 64 + chunk_place<PAIR_Q>(row, chunk) * 8));
+        }
+      }
+    }
+  };
+  if (FROM_LDS) fetch_rest();
   constexpr int READS = PLANES * (FM + FN), PRODUCTS = FM * FN * (SPLIT ? 3 : 1);
 #pragma unroll
   for (int k = 0; k < STAGES; k++)
@@ -506,6 +557,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   uint32_t step = 0, buffer = 0;
   auto after = [](uint32_t buffer) { return buffer + 1 == STAGES ? 0 : buffer + 1; };
   for (; step + STAGES * KS < last; step += KS, buffer = after(buffer)) {
+    add_rest_of(step + mine, buffer);
     read(buffer, 1);
     multiply(0);
     interleave<READS, PRODUCTS, 0>();
@@ -518,6 +570,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   }
   for (; step < last; step += KS, buffer = after(buffer)) {
     const bool busy = KS == 1 || step + mine < last;
+    if (busy) add_rest_of(step + mine, buffer);
     read(buffer, 1);
     if (busy) multiply(0);
     wait_loads<0>();
@@ -529,6 +582,19 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
     for (int x = 0; x < FM; x++)
 #pragma unroll
       for (int y = 0; y < FN; y++) acc[x][y] += low[x][y] * (1.f / kScaleLow);
+  }
+  if constexpr (REST && !FROM_LDS) {
+    fetch_rest();
+#pragma unroll
+    for (int x = 0; x < FM; x += 2) {
+      const uint32_t row = i0 + wi + x * 16;
+      if (row >= m) break;
+#pragma unroll
+      for (int y = 0; y < FN; y++) {
+        const uint32_t col = j0 + wj + row_of_piece<PAIR_Q>(y, lane % 16);
+        add_rest(x, y, *reinterpret_cast<const half8*>(at + y_hi + (static_cast<uint64_t>(col < n ? col : n - 1) * m + row + lane / 16 * 8) * 2));
+      }
+    }
   }
 
   // the groups' sums, in their order; each goes on with its share of the pieces of a place in the tile
@@ -631,6 +697,13 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
               } else {
                 v[e] *= 1.f / kScaleB;
                 if (with_low) v[e] += a * (1.f / kScaleLow) * static_cast<float>(old_lo[set % AHEAD][y][dx * 4 + e]);
+              }
+            }
+            if (KIND == SQUARE && !SPLIT && ti == tj) {
+              const uint32_t i = wi + set * 16 * DOWN + col_i + dx * 4, j = wj + ey * 16 + y0 * 16 + dy * 4 + col_j, e = j - i;
+              if (e < 4) {
+                const float on = e == 0 ? v[0] : e == 1 ? v[1] : e == 2 ? v[2] : v[3];
+                reinterpret_cast<_Float16*>(at + p.b_rest)[j0 + j] = static_cast<_Float16>(on - static_cast<float>(static_cast<_Float16>(on)));
               }
             }
             if constexpr (KIND == LAST) {
