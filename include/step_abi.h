@@ -93,8 +93,8 @@ int step_sum_slices(const void* ids, int id_type, size_t tokens, const void* val
  * precise = 0: the products take fp16 operands (the rest of the iterate is kept
  * beside them): the norm of the difference is 0.05 to 0.3 % of the result's, about
  * bfloat16's own rounding; up to 0.6 % with fewer than eight rows (or columns).
- * precise = 1: three products of split operands: about 1e-6 off; a list whose
- * matrices are all of at most 64 x 256 (or 256 x 64) always has these. Iterates must
+ * precise = 1: three products of split operands: about 1e-6 off; matrices of at
+ * most 64 x 256 (or 256 x 64) always have these, whatever else is in the list. Iterates must
  * stay below 64 in every entry and X X^T below 4, which coefficients that bring
  * singular values towards 1 see to. */
 typedef struct step_matrix {

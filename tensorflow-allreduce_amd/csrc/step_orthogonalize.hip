@@ -981,12 +981,16 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(SmallItems items, 
 // Elements of one round, beyond which more matrices fill the GPU no better and only ask for more workspace.
 constexpr uint64_t kRoundElements = 1ull << 26;
 
-// Whether all matrices of a list are small. Among larger ones they ride along in launches that are made anyway: of the
-// ResNet-50 set's 54 matrices 8 are small, and on their own they would take 98 us beside the 1370 of the whole step.
-bool all_small(const step_matrix* list, size_t length) {
-  for (size_t k = 0; k < length; k++)
-    if (std::min(list[k].rows, list[k].cols) > kSmallRows || std::max(list[k].rows, list[k].cols) > kSmallCols) return false;
-  return true;
+bool is_small(const step_matrix& x) { return std::min(x.rows, x.cols) <= kSmallRows && std::max(x.rows, x.cols) <= kSmallCols; }
+
+// Whether small matrices go with the larger ones of their list: with split products, as exact as on their own, they ride
+// along in launches that are made anyway (of the ResNet-50 set's 54 matrices 8 are small, and on their own they would take
+// 98 us beside the 1370 of the whole step). Products of single operands are for the larger ones only, or what a small
+// matrix gets would depend on its neighbours.
+bool rides_along(const step_matrix* list, size_t length, int precise) {
+  for (size_t k = 0; k < length && precise; k++)
+    if (!is_small(list[k])) return true;
+  return false;
 }
 
 struct Item {
@@ -994,9 +998,10 @@ struct Item {
   uint32_t m, n;
 };
 
-// Cuts the caller's list into rounds, their items in the order of their padded shapes; visit(items, their number) for each.
+// Cuts the caller's list (its small matrices only if asked to) into rounds, their items in the order of their padded
+// shapes; visit(items, their number) for each.
 template <typename Visit>
-int for_rounds(const step_matrix* list, size_t length, const Visit& visit) {
+int for_rounds(const step_matrix* list, size_t length, bool with_small, const Visit& visit) {
   Item items[kMostItems];
   int used = 0, shapes = 0;
   uint64_t elements = 0;
@@ -1010,7 +1015,7 @@ int for_rounds(const step_matrix* list, size_t length, const Visit& visit) {
   };
   for (size_t k = 0; k < length; k++) {
     const size_t rows = list[k].rows, cols = list[k].cols;
-    if (rows == 0 || cols == 0) continue;
+    if (rows == 0 || cols == 0 || (!with_small && is_small(list[k]))) continue;
     const uint32_t m = static_cast<uint32_t>(round_up(std::min(rows, cols), kPad));
     const uint32_t n = static_cast<uint32_t>(round_up(std::max(rows, cols), kPad));
     const uint64_t one = static_cast<uint64_t>(m) * n;
@@ -1209,7 +1214,7 @@ int run_round(const step_matrix* list, const Item* items, int count, int dtype, 
 
 constexpr uint32_t kMostGrid = 1u << 22;  // workgroups of a launch, whose lanes have to stay below 2^32
 
-// A list of small matrices, those of up to 64 x 128 apart: two workgroups of them fit a compute unit's LDS.
+// A list's small matrices, those of up to 64 x 128 apart: two workgroups of them fit a compute unit's LDS.
 int run_small(const step_matrix* list, size_t length, int dtype, int out_dtype, const Rule& rule, hipStream_t stream) {
   bool any = false;
   Coefficients coefficients;
@@ -1236,7 +1241,7 @@ int run_small(const step_matrix* list, size_t length, int dtype, int out_dtype, 
     };
     for (size_t k = 0; k < length; k++) {
       const step_matrix& x = list[k];
-      if (x.rows == 0 || x.cols == 0 || x.count == 0 || (std::max(x.rows, x.cols) <= 128) != (across == 128)) continue;
+      if (!is_small(x) || x.rows == 0 || x.cols == 0 || x.count == 0 || (std::max(x.rows, x.cols) <= 128) != (across == 128)) continue;
       for (size_t first = 0, take; first < x.count; first += take) {
         if (items.count == kMostItems || matrices == kMostGrid) flush();
         take = std::min<size_t>(x.count - first, kMostGrid - matrices);
@@ -1257,9 +1262,13 @@ int run(const step_matrix* list, size_t length, int dtype, int out_dtype, int pr
   if (rule.steps < 1 || rule.steps > kMostSteps || !rule.coefficients) return STEP_ERR_ARGUMENT;
   const size_t need = step_orthogonalize_workspace(list, length, precise);
   if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 256)) return STEP_ERR_ARGUMENT;
-  if (need == 0) return run_small(list, length, dtype, out_dtype, rule, stream);  // or nothing to do
+  const bool with_small = rides_along(list, length, precise);
+  if (!with_small) {
+    const int rc = run_small(list, length, dtype, out_dtype, rule, stream);
+    if (rc != STEP_OK) return rc;
+  }
   char* ws = static_cast<char*>(workspace);
-  return for_rounds(list, length, [&](const Item* items, int count) {
+  return for_rounds(list, length, with_small, [&](const Item* items, int count) {
     return precise ? run_round<true>(list, items, count, dtype, out_dtype, rule, ws, stream)
                    : run_round<false>(list, items, count, dtype, out_dtype, rule, ws, stream);
   });
@@ -1274,8 +1283,8 @@ extern "C" {
 
 size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int precise) {
   uint64_t most = 0;
-  if ((length && !list) || all_small(list, length)) return 0;
-  for_rounds(list, length, [&](const Item* items, int count) {
+  if (length && !list) return 0;
+  for_rounds(list, length, rides_along(list, length, precise), [&](const Item* items, int count) {
     most = std::max(most, layout_for(items, count, precise != 0).bytes);
     return static_cast<int>(STEP_OK);
   });

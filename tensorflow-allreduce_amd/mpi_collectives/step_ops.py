@@ -366,7 +366,8 @@ class Muon(torch.optim.Optimizer):
         adjust: what s is. "shape": sqrt(max(1, rows / cols)). "rms":
                 0.2 sqrt(max(rows, cols)), which gives the update the size that
                 Adam's usually has.
-        precise: as in `orthogonalize`; by default True for float32 weights.
+        precise: as in `orthogonalize`, matrix by matrix; by default True for
+                float32 weights.
     """
 
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5,

@@ -97,3 +97,26 @@ def test_the_documented_accuracy(shape, kind):
     want = exact_there(update)
     got = mpi.orthogonalize(update, dtype=torch.float32, precise=False)
     assert float((got.double() - want).norm() / want.norm()) <= (0.003 if min(shape) >= 8 else 0.006)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_a_small_matrix_is_as_exact_among_larger_ones(dtype):
+    """With products of single operands for the larger ones, a small one takes the same step as alone, bit for bit."""
+    shapes = [(64, 256), (300, 200), (20, 30), (65, 64), (128, 64), (64, 257), (2, 2)]
+    small = [s for s in shapes if min(s) <= 64 and max(s) <= 256]
+    make = lambda some: [torch.nn.Parameter(torch.zeros(s, dtype=dtype, device="cuda")) for s in some]  # noqa: E731
+    together, alone = make(shapes), make(small)
+    for params in (together, alone):
+        for p in params:
+            gen = torch.Generator().manual_seed(1000 * p.shape[0] + p.shape[1])
+            p.grad = torch.randn(*p.shape, generator=gen).to(dtype).cuda()
+    mpi.Muon(together, precise=False).step()
+    for p in alone:
+        mpi.Muon([p], precise=False).step()
+    for q in alone:
+        p, = [p for p in together if p.shape == q.shape]
+        assert torch.equal(p, q), p.shape
+    for p in together:
+        want = -0.02 * math.sqrt(max(1.0, p.shape[0] / p.shape[1])) * exact_there(p.grad)
+        off = float((p.detach().double() - want).norm() / want.norm())
+        assert off <= (1e-5 if tuple(p.shape) in small else 0.003) + torch.finfo(dtype).eps / 2
