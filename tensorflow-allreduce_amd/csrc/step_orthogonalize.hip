@@ -20,9 +20,9 @@
 // an update of rank one, and with it 0.05 to 0.3 % whatever the rank (norm of the
 // difference over that of the result; up to 0.6 % where an update has fewer than
 // eight rows, whose few roundings hit everything).
-//   SPLIT = false (16-bit results): products of the hi planes.
+//   SPLIT = false (bfloat16 results, 16-bit weights): products of the hi planes.
 //   (The last iterate but one does without: its rounding grows by a once.)
-//   SPLIT = true (float32 results): hi hi + (hi lo + lo hi) / 2048, three products,
+//   SPLIT = true (other results): hi hi + (hi lo + lo hi) / 2048, three products,
 //   22 bits of every operand: about 1e-6 off.
 //
 // Layout. Everything is padded to multiples of 64 with zeros, which the products
