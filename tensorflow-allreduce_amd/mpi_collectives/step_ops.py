@@ -11,6 +11,7 @@ import ctypes
 import math
 
 import torch
+from torch.autograd import forward_ad
 
 from . import step_abi
 from ._plugin import InvalidArgumentError
@@ -50,6 +51,16 @@ def _rows_of(t):
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         t = t.contiguous()
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
+
+
+def _is_dual(t):
+    """Whether t carries a tangent of forward-mode differentiation."""
+    return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
+
+
+def _in_memory(tangent):
+    """A tangent as the kernels read it: one that is known to be zero has no memory."""
+    return torch.zeros(tangent.shape, dtype=tangent.dtype, device=tangent.device) if tangent._is_zerotensor() else tangent
 
 
 # The current stream and device as plain numbers: these calls are a large part of a small operator's time, and in a
@@ -100,7 +111,7 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
 
     Sums are taken in 32 bits in the order of the tokens and rounded once to
     grad's type; the same call gives the same bits every time. The result is
-    differentiable with respect to grad."""
+    differentiable with respect to grad, backwards and forwards."""
     what = "embedding_gradient"
     _check_tensor(grad, "grad", _FLOATS, what)
     _check_tensor(ids, "ids", _IDS, what)
@@ -110,7 +121,7 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
         _refuse("%s: rows is %d", what, rows)
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         _refuse("%s: a gradient of shape %s for ids of shape %s", what, tuple(grad.shape), tuple(ids.shape))
-    if grad.requires_grad and torch.is_grad_enabled():
+    if grad.requires_grad and torch.is_grad_enabled() or _is_dual(grad):
         return _EmbeddingGradient.apply(grad, ids, rows, float(scale))
     return _gradient(grad, ids, rows, float(scale))
 
@@ -158,7 +169,7 @@ def sum_slices(slices):
     Sums are taken in 32 bits in the order of the rows and rounded once; the
     same call gives the same bits every time. The number of distinct indices is
     read from the GPU, so the call waits for its stream and cannot be captured
-    into a graph. No gradient flows through it."""
+    into a graph. No gradient flows through it, backwards or forwards."""
     what = "sum_slices"
     if not isinstance(slices, IndexedSlices):
         _refuse("%s: an IndexedSlices is needed, got %s", what, type(slices).__name__)
@@ -206,6 +217,7 @@ class _Embedding(torch.autograd.Function):
     @staticmethod
     def forward(ctx, ids, weight, scale, sparse):
         ctx.save_for_backward(ids)
+        ctx.save_for_forward(ids)
         ctx.set_materialize_grads(False)
         ctx.call = (weight.shape[0], scale, sparse)
         return _lookup(ids, weight, scale)
@@ -216,7 +228,7 @@ class _Embedding(torch.autograd.Function):
             return None, None, None, None
         rows, scale, sparse = ctx.call
         ids, = ctx.saved_tensors
-        if grad.requires_grad:
+        if grad.requires_grad or _is_dual(grad):
             return None, _EmbeddingGradient.apply(grad, ids, rows, scale), None, None
         if not sparse:
             return None, _gradient(grad, ids, rows, scale), None, None
@@ -226,6 +238,11 @@ class _Embedding(torch.autograd.Function):
         return None, torch.sparse_coo_tensor(index.long().unsqueeze(0), values, (rows, grad.shape[-1]),
                                              is_coalesced=True, check_invariants=False), None, None
 
+    @staticmethod
+    def jvp(ctx, _ids, tangent, _scale, _sparse):
+        ids, = ctx.saved_tensors
+        return embedding(ids, _in_memory(tangent), ctx.call[1])
+
 
 class _EmbeddingGradient(torch.autograd.Function):
     """The gradient as a function of its own, for gradients of gradients: it is linear, and its transpose the lookup."""
@@ -233,13 +250,19 @@ class _EmbeddingGradient(torch.autograd.Function):
     @staticmethod
     def forward(ctx, grad, ids, rows, scale):
         ctx.save_for_backward(ids)
-        ctx.scale = scale
+        ctx.save_for_forward(ids)
+        ctx.rows, ctx.scale = rows, scale
         return _gradient(grad, ids, rows, scale)
 
     @staticmethod
     def backward(ctx, grad):
         ids, = ctx.saved_tensors
         return embedding(ids, grad, ctx.scale), None, None, None
+
+    @staticmethod
+    def jvp(ctx, tangent, _ids, _rows, _scale):
+        ids, = ctx.saved_tensors
+        return embedding_gradient(_in_memory(tangent), ids, ctx.rows, ctx.scale)
 
 
 def embedding(ids, weight, scale=1.0, sparse=False):
@@ -258,7 +281,11 @@ def embedding(ids, weight, scale=1.0, sparse=False):
                 DistributedOptimizer exchanges as an IndexedSlices; its size
                 depends on the data, so that backward pass waits for its stream
                 and cannot be captured into a graph. Where gradients of
-                gradients are asked for (create_graph) it is dense all the same.
+                gradients are asked for (create_graph, or a gradient that carries
+                a tangent) it is dense all the same.
+
+    The lookup is linear in the table and differentiable backwards and, by
+    torch.autograd.forward_ad, forwards.
 
     A forward and backward pass can be captured into a graph. As with every
     function of torch, no eager graph of the same leaves may be alive then:
@@ -270,7 +297,7 @@ def embedding(ids, weight, scale=1.0, sparse=False):
     _same_device(what, ids, weight)
     if weight.dim() != 2:
         _refuse("%s: a table of shape %s; it has two dimensions", what, tuple(weight.shape))
-    if weight.requires_grad and torch.is_grad_enabled():
+    if weight.requires_grad and torch.is_grad_enabled() or _is_dual(weight):
         return _Embedding.apply(ids, weight, float(scale), bool(sparse))
     return _lookup(ids, weight, float(scale))
 
@@ -316,7 +343,7 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
                 256 (or the transposed) are always precise.
 
     An update with an infinity or NaN gives NaN. No gradient flows through the
-    result."""
+    result, backwards or forwards."""
     what = "orthogonalize"
     _check_tensor(update, "update", _FLOATS, what)
     if update.dim() < 2:

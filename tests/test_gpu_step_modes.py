@@ -1,0 +1,62 @@
+"""GPU tests of the step operators under the ways torch calls them: forward-mode
+differentiation."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import mpi_collectives as mpi
+from mpi_collectives import step_abi
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _gpu():
+    assert torch.cuda.is_available(), "these tests need the MI355X"
+    step_abi.lib()
+
+
+def values(seed, *shape, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed)).to(dtype).cuda()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_tangents(dtype):
+    """Both operators are linear: the tangent is the operator on the tangent, bit for bit, whatever its strides."""
+    ids = torch.randint(-1, 40, (3, 50), generator=torch.Generator().manual_seed(1)).cuda()
+    weight, grad = values(2, 40, 72, dtype=dtype), values(3, 3, 50, 72, dtype=dtype)
+    weight_tangent, grad_tangent = values(4, 72, 40, dtype=dtype).t(), values(5, 3, 72, 50, dtype=dtype).transpose(1, 2)
+    with forward_ad.dual_level():
+        for needed in (False, True):
+            w = forward_ad.make_dual(weight.clone().requires_grad_(needed), weight_tangent)
+            primal, moved = forward_ad.unpack_dual(mpi.embedding(ids, w, scale=3.0))
+            assert torch.equal(primal, mpi.embedding(ids, weight, scale=3.0))
+            assert torch.equal(moved, mpi.embedding(ids, weight_tangent, scale=3.0))
+            g = forward_ad.make_dual(grad.clone().requires_grad_(needed), grad_tangent)
+            primal, moved = forward_ad.unpack_dual(mpi.embedding_gradient(g, ids, 40, scale=3.0))
+            assert torch.equal(primal, mpi.embedding_gradient(grad, ids, 40, scale=3.0))
+            assert torch.equal(moved, mpi.embedding_gradient(grad_tangent, ids, 40, scale=3.0))
+
+
+def test_tangent_against_differences():
+    """Small powers of two: the difference quotient is exact."""
+    ids = torch.tensor([[2, 0, 2], [-1, 1, 2]]).cuda()
+    weight = torch.tensor([[1.0, 0.5], [2.0, -1.0], [0.25, 4.0]]).cuda()
+    tangent = torch.tensor([[2.0, 1.0], [0.0, -4.0], [0.5, 8.0]]).cuda()
+    with forward_ad.dual_level():
+        moved = forward_ad.unpack_dual(mpi.embedding(ids, forward_ad.make_dual(weight, tangent), scale=2.0)).tangent
+    quotient = (mpi.embedding(ids, weight + 0.25 * tangent, scale=2.0) - mpi.embedding(ids, weight, scale=2.0)) / 0.25
+    assert torch.equal(moved, quotient)
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_forward_over_backward(sparse):
+    """The gradient of sum(W[ids]^2) is 2 n W where n tokens have a row, its tangent 2 n t."""
+    ids = torch.tensor([2, 0, -1, 2]).cuda()
+    weight, tangent = values(6, 4, 24), values(7, 4, 24)
+    count = torch.tensor([[1.0], [0.0], [2.0], [0.0]]).cuda()
+    with forward_ad.dual_level():
+        w = weight.clone().requires_grad_(True)
+        out = mpi.embedding(ids, forward_ad.make_dual(w, tangent), sparse=sparse)
+        primal, moved = forward_ad.unpack_dual(torch.autograd.grad(out.square().sum(), w)[0])
+    assert torch.equal(primal, 2 * count * weight) and torch.equal(moved, 2 * count * tangent)

@@ -1,6 +1,11 @@
 """Host side of the step operators, without a GPU: what a list of matrices asks
 for, and what the Python entry points do before any kernel is launched."""
-from mpi_collectives import step_abi
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+import mpi_collectives as mpi
+from mpi_collectives import step_abi, step_ops
 
 
 def matrices(*shapes):
@@ -15,3 +20,68 @@ def test_small_matrices_need_no_workspace_among_larger_ones():
     assert lib.step_orthogonalize_workspace(mixed, 3, 1) > lib.step_orthogonalize_workspace(large, 1, 1) > 0
     for precise in (0, 1):
         assert lib.step_orthogonalize_workspace(matrices((64, 256), (20, 30)), 2, precise) == 0
+
+
+@pytest.fixture
+def plain(monkeypatch):
+    """The kernels of the lookup and its gradient as plain torch operations on the CPU, invisible to autograd."""
+    def lookup(ids, weight, scale):
+        inside = ((ids >= 0) & (ids < weight.shape[0])).unsqueeze(-1)
+        out = torch.where(inside, scale * weight.detach()[ids.clamp(0, weight.shape[0] - 1)], 0.0)
+        return torch.from_numpy(out.numpy().copy())
+
+    def gradient(grad, ids, rows, scale):
+        inside = (ids >= 0) & (ids < rows)
+        out = torch.zeros(rows, grad.shape[-1], dtype=grad.dtype).index_add(0, ids[inside], scale * grad.detach()[inside])
+        return torch.from_numpy(out.numpy().copy())
+
+    monkeypatch.setattr(step_ops, "_lookup", lambda *a: torch.no_grad()(lookup)(*a))
+    monkeypatch.setattr(step_ops, "_gradient", lambda *a: torch.no_grad()(gradient)(*a))
+    monkeypatch.setattr(step_ops, "_check_tensor", lambda *a: None)
+
+
+IDS = torch.tensor([[2, 0, -1], [2, 5, 1]])
+
+
+def test_forward_mode(plain):
+    """Both operators are linear: the tangent of the result is the operator on the tangent."""
+    weight, tangent = torch.randn(4, 3), torch.randn(4, 3)
+    grad, grad_tangent = torch.randn(2, 3, 3), torch.randn(2, 3, 3)
+    with forward_ad.dual_level():
+        for needed in (False, True):
+            w = forward_ad.make_dual(weight.clone().requires_grad_(needed), tangent)
+            primal, moved = forward_ad.unpack_dual(mpi.embedding(IDS, w, scale=2.0))
+            assert torch.equal(primal, mpi.embedding(IDS, weight, scale=2.0))
+            assert torch.equal(moved, mpi.embedding(IDS, tangent, scale=2.0))
+            g = forward_ad.make_dual(grad.clone().requires_grad_(needed), grad_tangent)
+            primal, moved = forward_ad.unpack_dual(mpi.embedding_gradient(g, IDS, 4, scale=2.0))
+            assert torch.equal(primal, mpi.embedding_gradient(grad, IDS, 4, scale=2.0))
+            assert torch.equal(moved, mpi.embedding_gradient(grad_tangent, IDS, 4, scale=2.0))
+        with torch.no_grad():
+            moved = forward_ad.unpack_dual(mpi.embedding(IDS, forward_ad.make_dual(weight, tangent))).tangent
+            assert torch.equal(moved, mpi.embedding(IDS, tangent))
+        assert forward_ad.unpack_dual(mpi.embedding(IDS, weight)).tangent is None
+        zero = torch._efficientzerotensor(4, 3)
+        assert not forward_ad.unpack_dual(mpi.embedding(IDS, forward_ad.make_dual(weight, zero))).tangent.any()
+
+
+@pytest.mark.parametrize("sparse", [False, True])
+def test_forward_over_backward(plain, sparse):
+    """A Hessian times a vector: the gradient of sum((2 W[ids])^3) is 24 n W^2 where n tokens have a row, its tangent 48 n W t."""
+    weight, tangent = torch.randn(4, 3, dtype=torch.float64), torch.randn(4, 3, dtype=torch.float64)
+    with forward_ad.dual_level():
+        w = weight.clone().requires_grad_(True)
+        out = mpi.embedding(IDS, forward_ad.make_dual(w, tangent), scale=2.0, sparse=sparse)
+        first, = torch.autograd.grad(out.pow(3).sum(), w)
+        primal, moved = forward_ad.unpack_dual(first)
+    count = torch.tensor([1.0, 1.0, 2.0, 0.0], dtype=torch.float64).unsqueeze(1)
+    assert torch.allclose(primal, 24 * count * weight ** 2) and torch.allclose(moved, 48 * count * weight * tangent)
+
+
+def test_backward_over_forward(plain):
+    """The tangent of the result is differentiable with respect to the table's tangent."""
+    weight, tangent = torch.randn(4, 3), torch.randn(4, 3, requires_grad=True)
+    with forward_ad.dual_level():
+        moved = forward_ad.unpack_dual(mpi.embedding(IDS, forward_ad.make_dual(weight, tangent), scale=2.0)).tangent
+    moved.sum().backward()
+    assert tangent.grad[:, 0].tolist() == [2.0, 2.0, 4.0, 0.0]
