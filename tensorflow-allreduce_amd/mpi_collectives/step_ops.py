@@ -5,7 +5,9 @@ matrix with the optimizer that uses it.
 
 They run on torch's current stream of the tensors' device, allocate through
 torch and synchronise nothing (except where a result's size depends on the
-data: sum_slices, and the sparse gradient of embedding).
+data: sum_slices, and the sparse gradient of embedding). torch.compile breaks
+its graph around them and runs them as they are; what records a trace instead
+(jit.trace, make_fx, torch.export) is refused.
 """
 import ctypes
 import math
@@ -30,6 +32,17 @@ class IndexedSlices:
 
 def _refuse(why, *args):
     raise InvalidArgumentError(why % args)
+
+
+_MODES = tuple(getattr(torch._C._TorchDispatchModeKey, k) for k in ("PROXY", "FAKE", "FUNCTIONAL"))
+
+
+def _check_run(what):
+    """Refuses to be traced. The kernels are launched past torch's dispatcher: a trace would hold the empty result and not
+    what fills it."""
+    if torch._C._get_tracing_state() is not None or torch._C._len_torch_dispatch_stack() and any(
+            torch._C._get_dispatch_mode(k) is not None for k in _MODES):
+        _refuse("%s: it launches kernels of its own, which a trace (jit.trace, make_fx, torch.export) does not hold", what)
 
 
 def _check_tensor(t, name, types, what):
@@ -113,6 +126,7 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
     grad's type; the same call gives the same bits every time. The result is
     differentiable with respect to grad, backwards and forwards."""
     what = "embedding_gradient"
+    _check_run(what)
     _check_tensor(grad, "grad", _FLOATS, what)
     _check_tensor(ids, "ids", _IDS, what)
     _same_device(what, grad, ids)
@@ -171,6 +185,7 @@ def sum_slices(slices):
     read from the GPU, so the call waits for its stream and cannot be captured
     into a graph. No gradient flows through it, backwards or forwards."""
     what = "sum_slices"
+    _check_run(what)
     if not isinstance(slices, IndexedSlices):
         _refuse("%s: an IndexedSlices is needed, got %s", what, type(slices).__name__)
     values, indices = slices.values, slices.indices
@@ -292,6 +307,7 @@ def embedding(ids, weight, scale=1.0, sparse=False):
     autograd would join its stream into the capture.
     """
     what = "embedding"
+    _check_run(what)
     _check_tensor(ids, "ids", _IDS, what)
     _check_tensor(weight, "weight", _FLOATS, what)
     _same_device(what, ids, weight)
@@ -345,6 +361,7 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
     An update with an infinity or NaN gives NaN. No gradient flows through the
     result, backwards or forwards."""
     what = "orthogonalize"
+    _check_run(what)
     _check_tensor(update, "update", _FLOATS, what)
     if update.dim() < 2:
         _refuse("%s: an update of shape %s; it has two dimensions at least", what, tuple(update.shape))
@@ -422,6 +439,7 @@ class Muon(torch.optim.Optimizer):
     @torch.no_grad()
     def step(self, closure=None):
         """One step for every parameter that has a gradient."""
+        _check_run("Muon.step")
         loss = None
         if closure is not None:
             with torch.enable_grad():

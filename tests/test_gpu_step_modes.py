@@ -1,5 +1,5 @@
 """GPU tests of the step operators under the ways torch calls them: forward-mode
-differentiation."""
+differentiation, torch.compile."""
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -60,3 +60,25 @@ def test_forward_over_backward(sparse):
         out = mpi.embedding(ids, forward_ad.make_dual(w, tangent), sparse=sparse)
         primal, moved = forward_ad.unpack_dual(torch.autograd.grad(out.square().sum(), w)[0])
     assert torch.equal(primal, 2 * count * weight) and torch.equal(moved, 2 * count * tangent)
+
+
+def test_compiled_around():
+    """torch.compile breaks its graph around the operators and runs them as they are."""
+    import torch._dynamo
+    torch._dynamo.reset()
+    ids = torch.tensor([[0, 2, -1, 2], [1, 1, 0, 3]]).cuda()
+    weight, update = values(8, 4, 24), values(9, 70, 90)
+
+    def step(ids, weight, update):
+        return (mpi.embedding(ids, weight * 2, scale=3.0) + 1).square().sum(), mpi.orthogonalize(update + 1) * 2
+
+    results = []
+    for f in (step, torch.compile(step, backend="eager")):
+        for _ in range(2):
+            leaf = weight.clone().requires_grad_(True)
+            loss, out = f(ids, leaf, update)
+            loss.backward()
+            results.append((loss.detach(), out, leaf.grad))
+    torch._dynamo.reset()
+    for r in results[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(r, results[0]))

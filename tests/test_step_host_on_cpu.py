@@ -85,3 +85,36 @@ def test_backward_over_forward(plain):
         moved = forward_ad.unpack_dual(mpi.embedding(IDS, forward_ad.make_dual(weight, tangent), scale=2.0)).tangent
     moved.sum().backward()
     assert tangent.grad[:, 0].tolist() == [2.0, 2.0, 4.0, 0.0]
+
+
+def _muon(weight):
+    opt = mpi.Muon([torch.nn.Parameter(weight)])
+    opt.step()
+    return weight
+
+
+@pytest.mark.parametrize("call", [
+    lambda x: mpi.embedding(IDS, x), lambda x: mpi.embedding(IDS, x.clone().requires_grad_(True)),
+    lambda x: mpi.embedding_gradient(x, torch.tensor([1, 0, 2, 2]), 5), lambda x: mpi.orthogonalize(x),
+    lambda x: mpi.sum_slices(mpi.IndexedSlices(x, torch.tensor([1, 0, 2, 2]), (4, 3))).values, _muon])
+def test_what_records_a_trace_is_refused(plain, call):
+    """A trace would hold the empty result and not the launch that fills it."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    from torch.fx.experimental.proxy_tensor import make_fx
+    x = torch.randn(4, 3)
+    for mode in ("real", "fake", "symbolic"):
+        with pytest.raises(mpi.InvalidArgumentError, match="does not hold"):
+            make_fx(call, tracing_mode=mode)(x)
+    with pytest.raises(mpi.InvalidArgumentError, match="does not hold"):
+        torch.jit.trace(call, x)
+    with FakeTensorMode(allow_non_fake_inputs=True), pytest.raises(mpi.InvalidArgumentError, match="does not hold"):
+        call(x)
+
+
+def test_other_modes_of_torch_are_none_of_a_trace(plain):
+    """Counting flops, say."""
+    from torch.utils.flop_counter import FlopCounterMode
+    weight = torch.randn(4, 3)
+    with FlopCounterMode(display=False):
+        out = mpi.embedding(IDS, weight)
+    assert torch.equal(out, mpi.embedding(IDS, weight))
