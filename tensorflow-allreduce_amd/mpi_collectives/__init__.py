@@ -693,7 +693,7 @@ class DistributedOptimizer:
       use_locking: accepted for signature compatibility.
       fusion: pack all dense float32 gradients into one fusion buffer and
         reduce them with a single ring allreduce (not in the reference, which
-        issues one allreduce per gradient).
+        issues one allreduce per gradient). Others are exchanged as without it.
     """
 
     def __init__(self, optimizer, name=None, use_locking=False, fusion=False):
@@ -733,14 +733,13 @@ class DistributedOptimizer:
         reduced = dict(zip((id(p) for p in dense), self._reduce_dense([p.grad for p in dense])))
         out = []
         for p in params:
-            g = p.grad
-            if g.is_sparse:
-                g = _coalesced(g)
-                slices = IndexedSlices(g.values().contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape)
-                out.append((allreduce(slices), p))
-            else:
-                out.append((reduced[id(p)], p))
+            out.append((self._reduce_sparse(p.grad) if p.grad.is_sparse else reduced[id(p)], p))
         return out
+
+    def _reduce_sparse(self, g):
+        """An averaged sparse gradient: the ranks' slices, one behind the other."""
+        g = _coalesced(g)
+        return allreduce(IndexedSlices(g.values().contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape))
 
     def _reduce_dense(self, grads):
         """Handles of the averaged dense gradients. A training loop presents the
@@ -776,10 +775,16 @@ class DistributedOptimizer:
         return self._batch.submit()
 
     def _compute_fused(self, params):
-        session, _ = mpi_ops._current()
         dense = [p for p in params if not p.grad.is_sparse and p.grad.dtype == torch.float32]
         dense_ids = {id(p) for p in dense}
-        rest = [p for p in params if id(p) not in dense_ids]
+        out = self._reduce_fused(dense) if dense else []
+        for p in params:
+            if id(p) not in dense_ids:
+                out.append((self._reduce_sparse(p.grad) if p.grad.is_sparse else allreduce(p.grad.contiguous()), p))
+        return out
+
+    def _reduce_fused(self, dense):
+        session, _ = mpi_ops._current()
         grads = [p.grad.contiguous() for p in dense]
         plan = ring_abi.FusionPlan([g.data_ptr() if g.numel() else None for g in grads],
                                    [g.numel() for g in grads], ring_abi.F32)
@@ -800,10 +805,7 @@ class DistributedOptimizer:
             return t
 
         session._after(handle, unpack)
-        out = [(_FusedGrad(handle, g), p) for g, p in zip(grads, dense)]
-        for p in rest:
-            out.append((allreduce(p.grad.contiguous()), p))
-        return out
+        return [(_FusedGrad(handle, g), p) for g, p in zip(grads, dense)]
 
     def apply_gradients(self, grads_and_vars, global_step=None, name=None):
         """Stores the reduced gradients on their variables and steps the
