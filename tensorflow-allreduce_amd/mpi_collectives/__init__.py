@@ -681,6 +681,19 @@ def _coalesced(g):
     return g.coalesce()
 
 
+_HALF = (torch.bfloat16, torch.float16)
+
+
+def _to_exchange(g):
+    """A gradient in a type that the collectives have."""
+    return g.float() if g.dtype in _HALF else g
+
+
+def _from_exchange(t, p):
+    """What came of _to_exchange, in the type of its variable."""
+    return t.to(p.dtype) if p.dtype in _HALF and t.dtype == torch.float32 else t
+
+
 class DistributedOptimizer:
     """An optimizer that wraps a torch.optim.Optimizer, using an MPI allreduce
     to average gradient values before applying gradients to model weights
@@ -691,9 +704,14 @@ class DistributedOptimizer:
       name: optional name prefix for the collectives this optimizer issues;
         defaults to "Distributed" followed by the optimizer's type.
       use_locking: accepted for signature compatibility.
-      fusion: pack all dense float32 gradients into one fusion buffer and
-        reduce them with a single ring allreduce (not in the reference, which
-        issues one allreduce per gradient). Others are exchanged as without it.
+      fusion: pack all dense floating-point gradients but float64 ones into one
+        fusion buffer and reduce them with a single ring allreduce (not in the
+        reference, which issues one allreduce per gradient). Others are exchanged
+        as without it.
+
+    The collectives' own types have no 16-bit ones. Gradients in bfloat16 or
+    float16 are exchanged in float32, which compute_gradients returns, and
+    apply_gradients rounds the average once, to the variable's type.
     """
 
     def __init__(self, optimizer, name=None, use_locking=False, fusion=False):
@@ -730,7 +748,8 @@ class DistributedOptimizer:
         # one MPIAllreduce per gradient, as in the reference (__init__.py:195-205); the dense ones
         # are submitted together
         dense = [p for p in params if not p.grad.is_sparse]
-        reduced = dict(zip((id(p) for p in dense), self._reduce_dense([p.grad for p in dense])))
+        reduced = dict(zip((id(p) for p in dense), self._reduce_dense([_to_exchange(p.grad) for p in dense],
+                                                                      moving=any(p.grad.dtype in _HALF for p in dense))))
         out = []
         for p in params:
             out.append((self._reduce_sparse(p.grad) if p.grad.is_sparse else reduced[id(p)], p))
@@ -739,15 +758,16 @@ class DistributedOptimizer:
     def _reduce_sparse(self, g):
         """An averaged sparse gradient: the ranks' slices, one behind the other."""
         g = _coalesced(g)
-        return allreduce(IndexedSlices(g.values().contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape))
+        return allreduce(IndexedSlices(_to_exchange(g.values()).contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape))
 
-    def _reduce_dense(self, grads):
+    def _reduce_dense(self, grads, moving=False):
         """Handles of the averaged dense gradients. A training loop presents the
         same gradient tensors every step, so their MPIAllreduce nodes are built
         once (the reference's graph) and run again while the tensors stay where
-        they are; anything else goes through allreduce_batch."""
+        they are; anything else (moving: copies of gradients) goes through
+        allreduce_batch."""
         session, _ = mpi_ops._current()
-        if session._immediate or not grads or not all(g.is_cuda and g.is_contiguous() for g in grads):
+        if session._immediate or not grads or moving or not all(g.is_cuda and g.is_contiguous() for g in grads):
             return allreduce_batch(grads)
         key = (id(session),) + tuple(g.data_ptr() for g in grads) + tuple(g.shape for g in grads)
         for old in [b for b in self._stale if b.completed]:
@@ -775,7 +795,7 @@ class DistributedOptimizer:
         return self._batch.submit()
 
     def _compute_fused(self, params):
-        dense = [p for p in params if not p.grad.is_sparse and p.grad.dtype == torch.float32]
+        dense = [p for p in params if not p.grad.is_sparse and p.grad.dtype in (torch.float32,) + _HALF]
         dense_ids = {id(p) for p in dense}
         out = self._reduce_fused(dense) if dense else []
         for p in params:
@@ -785,7 +805,7 @@ class DistributedOptimizer:
 
     def _reduce_fused(self, dense):
         session, _ = mpi_ops._current()
-        grads = [p.grad.contiguous() for p in dense]
+        grads = [_to_exchange(p.grad).contiguous() for p in dense]
         plan = ring_abi.FusionPlan([g.data_ptr() if g.numel() else None for g in grads],
                                    [g.numel() for g in grads], ring_abi.F32)
         fused = torch.empty(plan.elements, dtype=torch.float32, device="cuda")
@@ -816,14 +836,15 @@ class DistributedOptimizer:
             if isinstance(g, IndexedSlices):
                 if not _can_sum_slices(g):
                     idx = g.indices.reshape(1, -1)
-                    p.grad = torch.sparse_coo_tensor(idx, g.values, size=tuple(g.dense_shape)).coalesce()
+                    g = torch.sparse_coo_tensor(idx, g.values, size=tuple(g.dense_shape)).coalesce()
+                    p.grad = _from_exchange(g, p)
                     continue
                 # every rank's rows, one behind the other: one row for each index, the ranks' rows added in order
                 total = sum_slices(g)
-                p.grad = torch.sparse_coo_tensor(total.indices.long().reshape(1, -1), total.values,
+                p.grad = torch.sparse_coo_tensor(total.indices.long().reshape(1, -1), _from_exchange(total.values, p),
                                                  size=tuple(g.dense_shape), is_coalesced=True)
             else:
-                p.grad = g.reshape(p.shape)
+                p.grad = _from_exchange(g.reshape(p.shape), p)
         return self._optimizer.step()
 
     def minimize(self, loss, global_step=None, var_list=None):
