@@ -225,7 +225,9 @@ def _sum_slices(values, indices, rows, scale):
         indices.data_ptr(), _IDS[indices.dtype], tokens, flat.data_ptr(), _FLOATS[dtype], rows, width, stride, scale,
         out_ids.data_ptr(), out.data_ptr(), count.data_ptr(), ws.data_ptr(), size, _stream_of(index)), "sum_slices")
     n = count.item()
-    return out_ids[:n], out[:n].view((n,) + shape)
+    out_ids, out = out_ids[:n], out[:n].view((n,) + shape)
+    # a gradient lives until the next step: where it is less than half of what was set aside, it does not keep the rest alive
+    return (out_ids.clone(), out.clone()) if 2 * n < most else (out_ids, out)
 
 
 class _Embedding(torch.autograd.Function):

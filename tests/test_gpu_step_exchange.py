@@ -140,3 +140,19 @@ def test_muon_in_bfloat16_through_the_exchange(fusion):
         alone.step()
         for ws in weights:
             assert all(torch.equal(a, b) for a, b in zip(ws, mirror))
+
+
+@pytest.mark.parametrize("distinct", [1, 3, 300, 499, 500, 501, 999, 1000])
+def test_summed_slices_keep_no_more_than_twice_their_size(distinct):
+    """Every rank's rows are set aside for the sum; a gradient of few distinct rows must not keep them until the next step."""
+    count, width = 1000, 64
+    ids = torch.arange(count).remainder(distinct).cuda()
+    rows = values(50, count, width)
+    got = mpi.sum_slices(mpi.IndexedSlices(rows, ids, (5000, width)))
+    assert got.indices.tolist() == list(range(distinct)) and got.values.shape == (distinct, width)
+    for t in (got.indices, got.values):
+        assert t.is_contiguous() and t.untyped_storage().nbytes() <= 2 * t.numel() * t.element_size()
+    weight = values(51, 5000, width).requires_grad_(True)
+    mpi.embedding(ids, weight, sparse=True).backward(rows)
+    assert torch.equal(weight.grad._values(), got.values)
+    assert weight.grad._values().untyped_storage().nbytes() <= 2 * got.values.numel() * 4
