@@ -164,9 +164,15 @@ def _gradient(grad, ids, rows, scale):
 
 
 def can_sum_slices(slices):
-    """Whether sum_slices takes the tensors of `slices`: their types, on a GPU."""
-    return (slices.values.is_cuda and slices.values.dtype in _FLOATS and slices.indices.is_cuda and
-            slices.indices.dtype in _IDS and slices.indices.dim() == 1)
+    """Whether sum_slices takes the tensors of `slices`: their types, on a GPU, of sizes that fit its 32-bit places and its
+    launches. (A lane sums 16 bytes of the runs that begin in eight rows, and may have as many idle ones beside it: 2^36 bytes
+    of rows, of at least 16 each, are a quarter of the 2^32 lanes of a launch.)"""
+    values, indices = slices.values, slices.indices
+    if not (values.is_cuda and values.dtype in _FLOATS and indices.is_cuda and indices.dtype in _IDS and indices.dim() == 1):
+        return False
+    row = math.prod(values.shape[1:])
+    return (slices.dense_shape is not None and int(slices.dense_shape[0]) < 1 << 31 and row <= 65535 * 256 * 4 and
+            indices.shape[0] < 1 << 31 and indices.shape[0] * max(row * values.element_size(), 16) <= 1 << 36)
 
 
 def sum_slices(slices):

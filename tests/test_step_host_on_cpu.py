@@ -1,5 +1,8 @@
 """Host side of the step operators, without a GPU: what a list of matrices asks
 for, and what the Python entry points do before any kernel is launched."""
+import ctypes
+import types
+
 import pytest
 import torch
 from torch.autograd import forward_ad
@@ -118,3 +121,29 @@ def test_other_modes_of_torch_are_none_of_a_trace(plain):
     with FlopCounterMode(display=False):
         out = mpi.embedding(IDS, weight)
     assert torch.equal(out, mpi.embedding(IDS, weight))
+
+
+def _slices(rows, row, dense_rows, dtype=torch.float32):
+    """Stand-ins for tensors on the GPU that nothing reads."""
+    meta = lambda shape, kind: types.SimpleNamespace(  # noqa: E731
+        is_cuda=True, dtype=kind, shape=torch.Size(shape), dim=lambda: len(shape), element_size=lambda: kind.itemsize)
+    return mpi.IndexedSlices(meta((rows, row), dtype), meta((rows,), torch.int64), (dense_rows, row))
+
+
+@pytest.mark.parametrize("rows, row, dense_rows, dtype, fits", [
+    (5, 3, 7, torch.float32, True), (5, 3, 7, torch.float64, False),
+    (5, 3, (1 << 31) - 1, torch.float32, True), (5, 3, 1 << 31, torch.float32, False), (5, 3, 1 << 40, torch.float32, False),
+    ((1 << 31) - 1, 1, 9, torch.bfloat16, True), (1 << 31, 1, 9, torch.bfloat16, False),
+    (2, 67107840, 9, torch.float32, True), (2, 67107841, 9, torch.float32, False),
+    (1 << 24, 1024, 9, torch.float32, True), (1 << 27, 1024, 9, torch.float32, False), (1 << 28, 2048, 9, torch.bfloat16, False)])
+def test_slices_beyond_the_kernels_sizes_go_to_torch(rows, row, dense_rows, dtype, fits):
+    """apply_gradients asks can_sum_slices first; what it lets through, the entry point takes."""
+    slices = _slices(rows, row, dense_rows, dtype)
+    assert step_ops.can_sum_slices(slices) == fits
+    if fits:
+        code = {torch.float32: 0, torch.bfloat16: 3}[dtype]
+        status = step_abi.lib().step_sum_slices(4096, 2, rows, 4096, code, dense_rows, row, row, 1.0, 4096, 4096,
+                                                ctypes.c_void_p(4096), None, 0, None)
+        assert status == 2          # only the workspace is missing: the sizes passed
+    slices.dense_shape = None
+    assert not step_ops.can_sum_slices(slices)
