@@ -106,6 +106,10 @@ typedef struct step_matrix {
   float rate;        /* step_muon: learning rate of this batch's matrices */
 } step_matrix;
 
+/* The side of the tiles that a product of the first round of a list is cut into: product = 0 X X^T, 1 A A, 2 B X, 3 the
+ * last B X. 0 if the list takes no such product (it is empty, or its matrices are small). For tests and tuning. */
+int step_orthogonalize_side(const step_matrix* list, size_t length, int precise, int product);
+
 /* Bytes of workspace for a list: 0 if none is needed. */
 size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int precise);
 int step_orthogonalize(const step_matrix* list, size_t length, int dtype, int out_dtype, int precise, int steps,

@@ -1127,37 +1127,42 @@ void launch_product(const Groups& groups, uint32_t tiles, const Extra& targets, 
 // where there are few; the costs are those measured for one 1024 x 4096, 16 of 1024 x 1024, 4096 x 4096, 4096 x 16384 and
 // 8192 x 8192. The Gram matrix of 4096 x 16384 has 136 tiles of 256 (326 us), 253 of 192 (256 us) or 528 of 128 (355 us), that of
 // 1024 x 2752 has 36 of 128 (33 us) or 136 of 64 (17 us).
+template <Kind KIND, bool SPLIT> uint32_t side_for(Groups groups) {
+  constexpr bool SQUARES = KIND == APPLY || KIND == LAST;
+  uint32_t tiles;
+  if (SPLIT) {
+    const double large = cut<KIND>(groups, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
+    const double small = cut<KIND>(groups, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
+    return large < small ? 128 : 64;
+  }
+  uint64_t elements = 0;
+  for (int k = 0; k < groups.count; k++) elements += static_cast<uint64_t>(groups.at[k].m) * groups.at[k].n * groups.at[k].count;
+  const bool far = elements > kNearElements;
+  const double t256 = cut<KIND>(groups, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? (far ? 26. : 22.) : KIND == APPLY ? (far ? 35. : 28.) : 10., 1}, &tiles);
+  const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, 192, Cost{0.98, 5., 1}, &tiles);
+  const double t128 = cut<KIND>(groups, 128, Cost{0.98, KIND == LAST ? (far ? 14. : 8.) : KIND == APPLY ? (far ? 20. : 10.) : 4., 2}, &tiles);
+  const double t64 = cut<KIND>(groups, 64, Cost{0.17, 3.5, 1}, &tiles);
+  if (t64 <= std::min(std::min(t256, t192), t128)) return 64;
+  if (t128 <= std::min(t256, t192)) return 128;
+  return t256 <= t192 ? 256 : 192;
+}
+
 template <Kind KIND, bool SPLIT, typename Extra>
 void product(const Layout& l, const Extra& targets, char* ws, int from, int low_in, int low_out, const float* coefficients,
              hipStream_t stream) {
-  constexpr bool SQUARES = KIND == APPLY || KIND == LAST;
   Groups groups = l.groups;
+  const uint32_t side = side_for<KIND, SPLIT>(groups);
   uint32_t tiles;
-  auto go = [&](auto kernel, uint32_t side) {
-    cut<KIND>(groups, side, Cost{0, 0, 1}, &tiles);
-    kernel(groups, tiles);
-  };
-#define STEP_PRODUCT(...)                                                                                            \
-  [&](const Groups& g, uint32_t t) {                                                                                 \
-    launch_product<__VA_ARGS__, KIND, SPLIT>(g, t, targets, ws, from, low_in, low_out, coefficients, stream);        \
-  }
+  cut<KIND>(groups, side, Cost{0, 0, 1}, &tiles);
+#define STEP_PRODUCT(...) launch_product<__VA_ARGS__, KIND, SPLIT>(groups, tiles, targets, ws, from, low_in, low_out, coefficients, stream)
   if constexpr (SPLIT) {
-    const double large = cut<KIND>(groups, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
-    const double small = cut<KIND>(groups, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
-    if (large < small) go(STEP_PRODUCT(128, 2, 4, 1, 2), 128);
-    else go(STEP_PRODUCT(64, 2, 2, 2, 2), 64);
+    if (side == 128) STEP_PRODUCT(128, 2, 4, 1, 2);
+    else STEP_PRODUCT(64, 2, 2, 2, 2);
   } else {
-    uint64_t elements = 0;
-    for (int k = 0; k < groups.count; k++) elements += static_cast<uint64_t>(groups.at[k].m) * groups.at[k].n * groups.at[k].count;
-    const bool far = elements > kNearElements;
-    const double t256 = cut<KIND>(groups, 256, Cost{SQUARES ? 1.5 : 1.3, KIND == LAST ? (far ? 26. : 22.) : KIND == APPLY ? (far ? 35. : 28.) : 10., 1}, &tiles);
-    const double t192 = SQUARES ? 1e30 : cut<KIND>(groups, 192, Cost{0.98, 5., 1}, &tiles);
-    const double t128 = cut<KIND>(groups, 128, Cost{0.98, KIND == LAST ? (far ? 14. : 8.) : KIND == APPLY ? (far ? 20. : 10.) : 4., 2}, &tiles);
-    const double t64 = cut<KIND>(groups, 64, Cost{0.17, 3.5, 1}, &tiles);
-    if (t64 <= std::min(std::min(t256, t192), t128)) go(STEP_PRODUCT(64, 2, 2, 2, 4), 64);
-    else if (t128 <= std::min(t256, t192)) go(STEP_PRODUCT(128, 2, 2, 1, 2), 128);
-    else if (t256 <= t192) go(STEP_PRODUCT(256, 2, 4, 1, 2), 256);
-    else if constexpr (!SQUARES) go(STEP_PRODUCT(192, 2, 4, 1, 3), 192);
+    if (side == 64) STEP_PRODUCT(64, 2, 2, 2, 4);
+    else if (side == 128) STEP_PRODUCT(128, 2, 2, 1, 2);
+    else if (side == 256) STEP_PRODUCT(256, 2, 4, 1, 2);
+    else if constexpr (KIND == GRAM || KIND == SQUARE) STEP_PRODUCT(192, 2, 4, 1, 3);
   }
 #undef STEP_PRODUCT
 }
@@ -1289,6 +1294,22 @@ size_t step_orthogonalize_workspace(const step_matrix* list, size_t length, int 
     return static_cast<int>(STEP_OK);
   });
   return most;
+}
+
+int step_orthogonalize_side(const step_matrix* list, size_t length, int precise, int product) {
+  int side = 0;
+  if (length && !list) return 0;
+  for_rounds(list, length, rides_along(list, length, precise), [&](const Item* items, int count) {
+    const Groups groups = layout_for(items, count, precise != 0).groups;
+    auto of = [&](auto split) {
+      constexpr bool SPLIT = decltype(split)::value;
+      return product == GRAM ? side_for<GRAM, SPLIT>(groups) : product == SQUARE ? side_for<SQUARE, SPLIT>(groups)
+           : product == APPLY ? side_for<APPLY, SPLIT>(groups) : product == LAST ? side_for<LAST, SPLIT>(groups) : 0;
+    };
+    if (side == 0) side = static_cast<int>(precise ? of(std::true_type()) : of(std::false_type()));
+    return static_cast<int>(STEP_OK);
+  });
+  return side;
 }
 
 int step_orthogonalize(const step_matrix* list, size_t length, int dtype, int out_dtype, int precise, int steps,

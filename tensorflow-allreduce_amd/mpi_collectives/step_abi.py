@@ -19,7 +19,7 @@ EXPORTS = (
     "step_abi_version", "step_status_string", "step_last_hip_error",
     "step_embedding_lookup", "step_embedding_piece", "step_embedding_gradient_workspace", "step_embedding_gradient",
     "step_sum_slices_workspace", "step_sum_slices",
-    "step_orthogonalize_workspace", "step_orthogonalize", "step_muon",
+    "step_orthogonalize_side", "step_orthogonalize_workspace", "step_orthogonalize", "step_muon",
 )
 
 
@@ -63,6 +63,7 @@ def lib():
             "step_embedding_gradient": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp, sz, vp]),
             "step_sum_slices_workspace": (sz, [sz, sz, sz]),
             "step_sum_slices": (ci, [vp, ci, sz, vp, ci, sz, sz, sz, fl, vp, vp, vp, vp, sz, vp]),
+            "step_orthogonalize_side": (ci, [pm, sz, ci, ci]),
             "step_orthogonalize_workspace": (sz, [pm, sz, ci]),
             "step_orthogonalize": (ci, [pm, sz, ci, ci, ci, ci, pf, fl, vp, sz, vp]),
             "step_muon": (ci, [pm, sz, ci, ci, ci, pf, fl, fl, ci, fl, vp, sz, vp]),

@@ -147,3 +147,39 @@ def test_slices_beyond_the_kernels_sizes_go_to_torch(rows, row, dense_rows, dtyp
         assert status == 2          # only the workspace is missing: the sizes passed
     slices.dense_shape = None
     assert not step_ops.can_sum_slices(slices)
+
+
+# Batches of matrices and the sides of the tiles their products take (X X^T, A A, B X and the last B X), chosen so that
+# every kernel there is runs, with tiles that the matrix's edge cuts, in more than one step.
+TILES = {
+    ((1, 300, 500), False): (64, 64, 64, 64),
+    ((7, 1040, 1220), False): (128, 128, 128, 128),
+    ((1, 2731, 1000), False): (64, 64, 128, 128),
+    ((3, 1900, 2500), False): (128, 128, 256, 256),
+    ((3, 2220, 2230), False): (192, 192, 256, 256),
+    ((3, 2440, 2460), False): (256, 256, 128, 128),
+    ((1, 300, 500), True): (64, 64, 64, 64),
+    ((1, 1000, 2731), True): (64, 64, 128, 128),
+    ((3, 2220, 2400), True): (128, 128, 128, 128),
+    ((9, 1040, 1220), True): (128, 128, 128, 128),
+}
+
+
+@pytest.mark.parametrize("shape, precise", TILES)
+def test_sides_of_tiles(shape, precise):
+    lib, (count, rows, cols) = step_abi.lib(), shape
+    one = step_abi.Matrix(4096, None, 4096, rows, cols, count, 0.0)
+    assert tuple(lib.step_orthogonalize_side(one, 1, precise, k) for k in range(4)) == TILES[shape, precise]
+    assert lib.step_orthogonalize_side(one, 1, precise, 4) == 0
+
+
+def test_every_tile_there_is_has_a_test():
+    for precise, kernels in ((False, [{64, 128, 192, 256}, {64, 128, 192, 256}, {64, 128, 256}, {64, 128, 256}]), (True, [{64, 128}] * 4)):
+        for k, sides in enumerate(kernels):
+            assert {t[k] for (_, p), t in TILES.items() if p == precise} == sides
+
+
+def test_sides_of_nothing():
+    lib = step_abi.lib()
+    for m in (matrices((64, 256)), matrices((0, 500)), matrices()):
+        assert [lib.step_orthogonalize_side(m, len(m), 0, k) for k in range(4)] == [0] * 4
