@@ -49,8 +49,14 @@ constexpr float kScaleB = 1024.f;
 constexpr float kScaleLow = 2048.f;  // hi + lo / 2048: the next 11 bits, away from fp16's smallest numbers
 
 constexpr int kPad = 64;           // and the depth of one stage of a product
-constexpr int kMostItems = 64;     // batches of matrices of one round, by value in the kernels' arguments
-constexpr int kMostGroups = 32;    // and shapes among them
+// (a build for the CPU takes shorter rounds)
+#ifndef STEP_MOST_ITEMS
+#define STEP_MOST_ITEMS 64
+#define STEP_MOST_GROUPS 32
+#define STEP_ROUND_ELEMENTS (1ull << 26)
+#endif
+constexpr int kMostItems = STEP_MOST_ITEMS;    // batches of matrices of one round, by value in the kernels' arguments
+constexpr int kMostGroups = STEP_MOST_GROUPS;  // and shapes among them
 constexpr int kMostPieces = 1024;  // partial sums of squares per matrix
 constexpr uint64_t kPiece = 8192;  // elements of one, at least
 
@@ -304,9 +310,13 @@ enum Kind { GRAM, SQUARE, APPLY, LAST };
 
 // Moves 16 bytes per lane from global memory into LDS at base + 16 * lane, without registers in between.
 __device__ __forceinline__ void load_to_lds(const void* from, void* base) {
+#if defined(__HIP_DEVICE_COMPILE__)
   __builtin_amdgcn_global_load_lds(reinterpret_cast<const __attribute__((address_space(1))) uint32_t*>(reinterpret_cast<uintptr_t>(from)),
                                    reinterpret_cast<__attribute__((address_space(3))) uint32_t*>(static_cast<uint32_t>(reinterpret_cast<uintptr_t>(base))),
                                    16, 0, 0);
+#elif defined(STEP_MATRIX_SHIM_H_)
+  step_matrix_shim::load_to_lds(from, base);
+#endif
 }
 
 // Which row of a wave's part of a tile lane r of 16 reads for piece x. In pairs, so that the four rows of a result that a
@@ -332,7 +342,11 @@ template <int READS, int PRODUCTS, int LOADS> __device__ __forceinline__ void in
 }
 
 template <int N> __device__ __forceinline__ void wait_loads() {
+#if defined(__HIP_DEVICE_COMPILE__)
   asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+#elif defined(STEP_MATRIX_SHIM_H_)
+  step_matrix_shim::wait_loads(N);
+#endif
 }
 
 // Four lanes side by side hold four rows of one column each; afterwards four columns of one row each.
@@ -979,7 +993,7 @@ __global__ void __launch_bounds__(kSmallThreads) small_kernel(SmallItems items, 
 // ---- host side -----------------------------------------------------------------------
 
 // Elements of one round, beyond which more matrices fill the GPU no better and only ask for more workspace.
-constexpr uint64_t kRoundElements = 1ull << 26;
+constexpr uint64_t kRoundElements = STEP_ROUND_ELEMENTS;
 
 bool is_small(const step_matrix& x) { return std::min(x.rows, x.cols) <= kSmallRows && std::max(x.rows, x.cols) <= kSmallCols; }
 
@@ -1130,6 +1144,9 @@ void launch_product(const Groups& groups, uint32_t tiles, const Extra& targets, 
 template <Kind KIND, bool SPLIT> uint32_t side_for(Groups groups) {
   constexpr bool SQUARES = KIND == APPLY || KIND == LAST;
   uint32_t tiles;
+#if defined(STEP_MATRIX_SHIM_H_)
+  if (step_matrix_shim::g_side) return SPLIT ? std::min(step_matrix_shim::g_side, 128u) : SQUARES && step_matrix_shim::g_side == 192 ? 256 : step_matrix_shim::g_side;
+#endif
   if (SPLIT) {
     const double large = cut<KIND>(groups, 128, Cost{1.17, KIND == LAST ? 8. : KIND == APPLY ? 12. : 6., 1}, &tiles);
     const double small = cut<KIND>(groups, 64, Cost{0.48, KIND == APPLY ? 4. : 2.4, 1}, &tiles);
