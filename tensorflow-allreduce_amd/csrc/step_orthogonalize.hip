@@ -517,53 +517,46 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
         }
       }
   };
-  // What B's diagonal lost, as diagonal matrices of 32 rows (a pair of pieces), times those rows of X. Tiles of up to 128 take
-  // them from LDS while their stage is there; of 256 once more from the L2 behind the last one, as a branch in the main loop
-  // costs them their registers. (B X of 16 1024 x 1024: 53.1 us without, 58.4 all
-  // from the L2, 56.4 from LDS.)
-  constexpr bool REST = FROM_Y && !SPLIT, FROM_LDS = SIDE < 256;
+  // What B's diagonal lost, as diagonal matrices of 32 rows (a pair of pieces), times those rows of X, from LDS while their
+  // stage is there. (Muon of 24 matrices of width 1024: 1683 us without, 1713 so, 1760 with those rows fetched once more
+  // behind the last stage.)
+  constexpr bool REST = FROM_Y && !SPLIT;
   static_assert(!REST || PAIR_P, "");
-  const uint32_t rest_row = lane % 16 / 4 * 8 + lane % 4;
-  _Float16 rest[REST ? FM : 1];
-  auto fetch_rest = [&]() {
+  __shared__ uint16_t rest[REST ? SIDE : 1];
+  uint32_t one_rest = 0;
+  if (REST && threadIdx.x < SIDE) one_rest = reinterpret_cast<const uint16_t*>(at + p.b_rest)[i0 + threadIdx.x < m ? i0 + threadIdx.x : m - 1];
+  auto add_rest = [&](uint32_t stage, uint32_t buffer) {
     if constexpr (REST) {
 #pragma unroll
       for (int x = 0; x < FM; x++) {
-        const uint32_t row = i0 + wi + x / 2 * 32 + x % 2 * 4 + rest_row;
-        rest[x] = reinterpret_cast<const _Float16*>(at + p.b_rest)[row < m ? row : m - 1];
-      }
-    }
-  };
-  auto add_rest = [&](int x, int y, half8 q) {
-    half8 d0 = {}, d1 = {};
-#pragma unroll
-    for (uint32_t e = 0; e < 4; e++) {
-      const bool here = lane / 16 == lane % 16 / 4 && lane % 4 == e;
-      d0[e] = here ? rest[x] : static_cast<_Float16>(0);
-      d1[e + 4] = here ? rest[x + 1] : static_cast<_Float16>(0);
-    }
-    acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d0, q, acc[x][y], 0, 0, 0);
-    acc[x + 1][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(d1, q, acc[x + 1][y], 0, 0, 0);
-  };
-  auto add_rest_of = [&](uint32_t stage, uint32_t buffer) {
-    if constexpr (REST && FROM_LDS) {
-#pragma unroll
-      for (int x = 0; x < FM; x += 2) {
-        const uint32_t half = (i0 + wi) / 32 + x / 2, chunk = half % 2 * 4 + lane / 16;
+        const uint32_t half = (i0 + wi) / 32 + x / 2;
         if (half / 2 != stage) continue;
+        uint32_t lane = threadIdx.x % 64;
+#if defined(__HIP_DEVICE_COMPILE__)
+        asm volatile("" : "+v"(lane));  // the diagonals are made here: kept through the loop, they cost tiles of 256 their registers
+#endif
+        // the lane's row of the piece is on the diagonal in one of the eight places that the lane holds of it, or in none
+        const uint32_t chunk = half % 2 * 4 + lane / 16, place = lane % 4;
+        uint32_t on = rest[wi + row_of_piece<true>(x, lane % 16)];
+        on = lane / 16 == lane % 16 / 4 ? place % 2 ? on << 16 : on : 0;
+        typedef uint32_t raw4 __attribute__((ext_vector_type(4)));
+        raw4 d = {0, 0, 0, 0};
+        d[x % 2 * 2] = place < 2 ? on : 0;
+        d[x % 2 * 2 + 1] = place < 2 ? 0 : on;
 #pragma unroll
         for (int y = 0; y < FN; y++) {
           const uint32_t row = wj + row_of_piece<PAIR_Q>(y, lane % 16);
-          add_rest(x, y, *reinterpret_cast<const half8*>(lds + (buffer * KS + mine) * SUB + (SIDE + row) * 64 + chunk_place<PAIR_Q>(row, chunk) * 8));
+          const half8 q = *reinterpret_cast<const half8*>(lds + (buffer * KS + mine) * SUB + (SIDE + row) * 64 + chunk_place<PAIR_Q>(row, chunk) * 8);
+          acc[x][y] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(half8, d), q, acc[x][y], 0, 0, 0);
         }
       }
     }
   };
-  if (FROM_LDS) fetch_rest();
   constexpr int READS = PLANES * (FM + FN), PRODUCTS = FM * FN * (SPLIT ? 3 : 1);
 #pragma unroll
   for (int k = 0; k < STAGES; k++)
     if (static_cast<uint32_t>(k * KS) < last) issue(k * KS, k);
+  if (REST && threadIdx.x < SIDE) rest[threadIdx.x] = static_cast<uint16_t>(one_rest);
   // the first stage has landed when at most the later ones' loads are under way
   if ((STAGES - 1) * KS < last) wait_loads<(STAGES - 1) * LOADS>();
   else wait_loads<0>();
@@ -571,7 +564,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   uint32_t step = 0, buffer = 0;
   auto after = [](uint32_t buffer) { return buffer + 1 == STAGES ? 0 : buffer + 1; };
   for (; step + STAGES * KS < last; step += KS, buffer = after(buffer)) {
-    add_rest_of(step + mine, buffer);
+    add_rest(step + mine, buffer);
     read(buffer, 1);
     multiply(0);
     interleave<READS, PRODUCTS, 0>();
@@ -584,7 +577,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
   }
   for (; step < last; step += KS, buffer = after(buffer)) {
     const bool busy = KS == 1 || step + mine < last;
-    if (busy) add_rest_of(step + mine, buffer);
+    if (busy) add_rest(step + mine, buffer);
     read(buffer, 1);
     if (busy) multiply(0);
     wait_loads<0>();
@@ -597,20 +590,6 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
 #pragma unroll
       for (int y = 0; y < FN; y++) acc[x][y] += low[x][y] * (1.f / kScaleLow);
   }
-  if constexpr (REST && !FROM_LDS) {
-    fetch_rest();
-#pragma unroll
-    for (int x = 0; x < FM; x += 2) {
-      const uint32_t row = i0 + wi + x * 16;
-      if (row >= m) break;
-#pragma unroll
-      for (int y = 0; y < FN; y++) {
-        const uint32_t col = j0 + wj + row_of_piece<PAIR_Q>(y, lane % 16);
-        add_rest(x, y, *reinterpret_cast<const half8*>(at + y_hi + (static_cast<uint64_t>(col < n ? col : n - 1) * m + row + lane / 16 * 8) * 2));
-      }
-    }
-  }
-
   // the groups' sums, in their order; each goes on with its share of the pieces of a place in the tile
   const uint32_t ey = mine * EN;
   float4v sum[FM][EN];
@@ -782,7 +761,7 @@ __global__ void __launch_bounds__(KS * WM * WN * 64, 2)
 
 // Matrices of at most 64 x 256 (or the transposed) are a workgroup each, from the momentum to the result in one launch:
 // both forms of X, A and B stay in LDS, every operand split. What bounds them is the chain of barriers and LDS reads of a
-// step (about 2 us), where the launches of the products above take 15: 48 of 64 x 128 21 us, by the products 78.
+// step (about 4 us), where the launches of the products above take 15: 48 of 64 x 128 21 us, by the products 78.
 constexpr uint32_t kSmallRows = 64, kSmallCols = 256, kSmallThreads = 512;
 
 struct SmallItem {
