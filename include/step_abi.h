@@ -40,7 +40,7 @@ enum step_status {
   STEP_ERR_HIP = 3,      /* a HIP runtime call failed: step_last_hip_error() */
   STEP_ERR_LIMIT = 5     /* more than 2^31 - 1 tokens or rows, 67,107,840 columns, or 2^32 - 1 lanes of a launch:
                             2^26 tokens of a lookup of rows of 4 KiB, 2^27 of their gradient (half as many at 8 KiB),
-                            2^30 rows of a gradient */
+                            2^30 rows of a gradient; a matrix to orthogonalise of more than 2^20 a side or 2^33 entries */
 };
 
 int step_abi_version(void);

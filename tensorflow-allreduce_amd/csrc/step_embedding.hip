@@ -166,7 +166,7 @@ struct Digits {
   int bits, passes;
 };
 
-// Digits of at most 9 bits: a table of up to 2^18 rows takes two passes.
+// Digits of at most 9 bits: a table of fewer than 2^18 rows takes two passes (the key `rows` needs bits too).
 Digits digits_for(size_t rows) {
   int bits = 1;
   while (bits < 32 && (rows >> bits) != 0) bits++;
@@ -424,8 +424,7 @@ __global__ void __launch_bounds__(kSortThreads) scatter_kernel(const void* ids, 
   }
 }
 
-// The runs of the sorted keys. counts == nullptr: begin/end by key. Otherwise a run's number is its rank: a first
-// launch (number == 0) counts the runs that begin in each tile, a second numbers them.
+// The runs of the sorted keys: where each key's begins and ends (gradient).
 __global__ void __launch_bounds__(kSortThreads) runs_kernel(const uint32_t* keys, uint32_t tokens, uint32_t rows,
                                                             Sorted to) {
   const uint64_t i = static_cast<uint64_t>(blockIdx.x) * kSortThreads + threadIdx.x;
@@ -442,6 +441,7 @@ __device__ __forceinline__ bool begins_run(const uint32_t* keys, uint64_t i, uin
   return key < rows && (i == 0 || keys[i - 1] != key);
 }
 
+// Runs by number (sum_slices): one launch counts those that begin in each tile, the next numbers them.
 __global__ void __launch_bounds__(kSortThreads) count_runs_kernel(const uint32_t* keys, uint32_t tokens, uint32_t rows,
                                                                   uint32_t tile_length, uint32_t* counts) {
   __shared__ RankScratch s;
@@ -811,7 +811,7 @@ Layout layout_for(size_t tokens, size_t rows, size_t width, bool numbered) {
   return l;
 }
 
-// Sorts the tokens and finds their runs. *numbered: see Sorted.
+// Sorts the tokens and finds their runs, by number (sum_slices) or by key: see Sorted.
 Sorted sort_tokens(const Layout& l, char* ws, const void* ids, int id_type, uint32_t tokens, uint32_t rows, bool numbered,
                    void* out_ids, int64_t* out_count, hipStream_t stream) {
   auto at = [ws](size_t offset) { return reinterpret_cast<uint32_t*>(ws + offset); };
@@ -929,7 +929,8 @@ const char* step_status_string(int status) {
     case STEP_ERR_DTYPE: return "Invalid tensor type passed.";
     case STEP_ERR_ARGUMENT: return "invalid argument";
     case STEP_ERR_HIP: return "HIP runtime call failed";
-    case STEP_ERR_LIMIT: return "more than 2^31 - 1 tokens or rows, 67107840 columns, or 2^32 - 1 lanes of a launch";
+    case STEP_ERR_LIMIT: return "more than 2^31 - 1 tokens, rows or matrices, 67107840 columns, 2^32 - 1 lanes of a launch, "
+                                "or a matrix to orthogonalize of more than 2^20 a side or 2^33 entries";
     default: return "unknown status";
   }
 }
