@@ -757,8 +757,8 @@ class DistributedOptimizer:
 
     def _reduce_sparse(self, g):
         """An averaged sparse gradient: the ranks' slices, one behind the other."""
-        g = _coalesced(g)
-        return allreduce(IndexedSlices(_to_exchange(g.values()).contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape))
+        g = _coalesced(_to_exchange(g))      # first, so that repeated indices are summed in 32 bits
+        return allreduce(IndexedSlices(g.values().contiguous(), g.indices()[0].contiguous(), dense_shape=g.shape))
 
     def _reduce_dense(self, grads, moving=False):
         """Handles of the averaged dense gradients. A training loop presents the

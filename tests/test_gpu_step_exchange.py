@@ -156,3 +156,17 @@ def test_summed_slices_keep_no_more_than_twice_their_size(distinct):
     mpi.embedding(ids, weight, sparse=True).backward(rows)
     assert torch.equal(weight.grad._values(), got.values)
     assert weight.grad._values().untyped_storage().nbytes() <= 2 * got.values.numel() * 4
+
+
+@pytest.mark.parametrize("fusion", [False, True])
+def test_repeated_indices_of_a_16_bit_gradient_are_summed_in_32(fusion):
+    """torch's own sparse gradient holds a row per token: 300 ones are 300, not the 256 where bfloat16 stops counting."""
+    weights = [torch.zeros(3, 8, dtype=torch.bfloat16, device="cuda").requires_grad_(True) for _ in range(2)]
+    opts = [mpi.DistributedOptimizer(torch.optim.SGD([w], lr=1.0), fusion=fusion) for w in weights]
+
+    def fill(r):
+        torch.nn.functional.embedding(torch.zeros(300, dtype=torch.int64).cuda(), weights[r], sparse=True).sum().backward()
+
+    exchange(2, opts, weights, fill)
+    for w in weights:
+        assert torch.equal(w.detach().cpu(), torch.tensor([[-300.0], [0.0], [0.0]]).expand(3, 8).bfloat16())
