@@ -134,3 +134,38 @@ def test_a_float16_result_is_as_exact_as_its_type(shape):
         off = float((got.double() - want).norm())
         assert off <= (1e-5 + 2.0 ** -11) * float(want.norm()) + 2.0 ** -25 * math.sqrt(want.numel())
     assert torch.equal(got, mpi.orthogonalize(update, dtype=torch.float16, precise=True))
+
+
+def test_a_mixed_list_captured_and_replayed():
+    """Small matrices and larger ones of one 16-bit list: their launches go into the graph together. Four replays with new
+    gradients against the same steps taken eagerly."""
+    shapes = [(64, 256), (300, 200), (20, 30), (128, 64), (64, 300)]
+    make = lambda: [torch.nn.Parameter(torch.ones(s, dtype=torch.bfloat16, device="cuda")) for s in shapes]  # noqa: E731
+    captured, eager = make(), make()
+    first, second = mpi.Muon(captured, weight_decay=0.1), mpi.Muon(eager, weight_decay=0.1)
+
+    def fill(seed):
+        for k, (p, q) in enumerate(zip(captured, eager)):
+            new = torch.randn(*p.shape, generator=torch.Generator().manual_seed(10 * seed + k)).bfloat16().cuda()
+            p.grad.copy_(new)
+            q.grad.copy_(new)
+
+    for p in captured + eager:
+        p.grad = torch.zeros_like(p)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        fill(0)
+        first.step(), second.step()
+        with torch.cuda.graph(graph, stream=side):
+            first.step()
+    torch.cuda.synchronize()
+    for seed in range(1, 5):
+        fill(seed)
+        torch.cuda.synchronize()
+        graph.replay()
+        second.step()
+        torch.cuda.synchronize()
+        for p, q in zip(captured, eager):
+            assert torch.equal(p, q) and torch.equal(first.state[p]["momentum_buffer"], second.state[q]["momentum_buffer"])
