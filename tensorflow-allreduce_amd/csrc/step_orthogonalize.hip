@@ -416,8 +416,8 @@ __device__ __forceinline__ void square_tile(uint32_t t, uint32_t down, uint32_t 
 // which take the stages of 64 halves of depth in turn and add their sums up in LDS at the end (tiles of 64: a matrix
 // has few, and its depth is what takes the time). Stages go from global memory into LDS without registers, STAGES deep;
 // the reads of a half step are mixed among the products of the half before.
-// Reached: the Gram matrix of 4096 x 16384 256 us (1075 TFLOP/s of its triangle), B X of the same 532 us (1033), of
-// 4096 x 4096 124 us (1109); 8192^3 by the library 1254. Behind the main loop every result is split, transposed and stored
+// Reached: the Gram matrix of 4096 x 16384 260 us (1057 TFLOP/s of its triangle), B X of the same 531 to 561 us (980 to
+// 1035); 8192^3 by the library 1254. Behind the main loop every result is split, transposed and stored
 // twice (8 to 16 bytes per element), with one workgroup on a compute unit and nothing to hide it behind: that bounds B X
 // where the contraction is short (m <= 1024, half of its time or more). Storing past the caches makes it slower (64-byte
 // pieces of lines, which the L2 joins), as does a contraction cut among workgroups that add up behind the last.
