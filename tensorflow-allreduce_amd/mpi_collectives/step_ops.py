@@ -66,6 +66,11 @@ def _rows_of(t):
     return t, (t.stride(0) if t.shape[0] > 1 else t.shape[1])
 
 
+def _as_stored(t):
+    """t with the values that its memory holds: a view can stand for the negative of them (the imaginary part of a conjugate)."""
+    return t.resolve_neg() if t.is_neg() else t
+
+
 def _is_dual(t):
     """Whether t carries a tangent of forward-mode differentiation."""
     return forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None
@@ -133,6 +138,7 @@ def embedding_gradient(grad, ids, rows, scale=1.0):
     rows = int(rows)
     if rows < 0:
         _refuse("%s: rows is %d", what, rows)
+    grad = _as_stored(grad)
     if grad.dim() != ids.dim() + 1 or grad.shape[:-1] != ids.shape:
         _refuse("%s: a gradient of shape %s for ids of shape %s", what, tuple(grad.shape), tuple(ids.shape))
     if grad.requires_grad and torch.is_grad_enabled() or _is_dual(grad):
@@ -198,6 +204,7 @@ def sum_slices(slices):
     _check_tensor(values, "values", _FLOATS, what)
     _check_tensor(indices, "indices", _IDS, what)
     _same_device(what, values, indices)
+    values = _as_stored(values)
     if slices.dense_shape is None:
         _refuse("%s: dense_shape is needed", what)
     shape = tuple(int(d) for d in slices.dense_shape)
@@ -251,6 +258,7 @@ class _Embedding(torch.autograd.Function):
             return None, None, None, None
         rows, scale, sparse = ctx.call
         ids, = ctx.saved_tensors
+        grad = _as_stored(grad)
         if grad.requires_grad or _is_dual(grad):
             return None, _EmbeddingGradient.apply(grad, ids, rows, scale), None, None
         if not sparse:
@@ -319,6 +327,7 @@ def embedding(ids, weight, scale=1.0, sparse=False):
     _check_tensor(ids, "ids", _IDS, what)
     _check_tensor(weight, "weight", _FLOATS, what)
     _same_device(what, ids, weight)
+    weight = _as_stored(weight)
     if weight.dim() != 2:
         _refuse("%s: a table of shape %s; it has two dimensions", what, tuple(weight.shape))
     if weight.requires_grad and torch.is_grad_enabled() or _is_dual(weight):
@@ -381,7 +390,7 @@ def orthogonalize(update, steps=5, coefficients=NEWTON_SCHULZ, eps=1e-7, dtype=N
     index = update.get_device()
     if index != _current_device():
         return _on_device(orthogonalize, update, update, steps, coefficients, eps, dtype, precise)
-    update = update.detach().contiguous()
+    update = _as_stored(update.detach()).contiguous()
     out = _empty(update.shape, dtype=dtype, device=update.device)
     rows, cols = update.shape[-2:]
     count = update.numel() // (rows * cols) if update.numel() else 0
@@ -470,6 +479,8 @@ class Muon(torch.optim.Optimizer):
         moved, keep = [], []      # weights that are not contiguous, with the copies that take the step; tensors in use
         for p, row in zip(params, table):
             g = p.grad
+            if p.is_neg():
+                _refuse("Muon: a weight that stands for the negative of its memory (resolve_neg makes one that does not)")
             if g.is_sparse:
                 _refuse("Muon: a sparse gradient; it takes matrices with dense ones")
             if g.dtype != dtype or g.device != device:
@@ -487,8 +498,8 @@ class Muon(torch.optim.Optimizer):
             if not p.is_contiguous():
                 w = p.contiguous()
                 moved.append((p, w))
-            if not g.is_contiguous():
-                g = g.contiguous()
+            if not g.is_contiguous() or g.is_neg():
+                g = _as_stored(g).contiguous()
                 keep.append(g)
             rows, cols = p.shape
             row.grad, row.momentum, row.out = g.data_ptr(), m.data_ptr(), w.data_ptr()

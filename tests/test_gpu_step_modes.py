@@ -82,3 +82,28 @@ def test_compiled_around():
     torch._dynamo.reset()
     for r in results[1:]:
         assert all(torch.equal(a, b) for a, b in zip(r, results[0]))
+
+
+def test_views_that_stand_for_the_negative_of_their_memory():
+    """The imaginary part of a conjugate, of one column: its memory holds the other sign at any stride the kernels take."""
+    z = torch.complex(values(10, 30, 1), values(11, 30, 1))
+    ids = torch.randint(-1, 30, (50,), generator=torch.Generator().manual_seed(12)).cuda()
+    view, plain = z.conj().imag, -z.imag
+    assert view.is_neg()
+    assert torch.equal(mpi.embedding(ids, view), mpi.embedding(ids, plain))
+    index = torch.arange(30).remainder(7).cuda()
+    assert torch.equal(mpi.embedding_gradient(view, index, 7), mpi.embedding_gradient(plain, index, 7))
+    got, want = (mpi.sum_slices(mpi.IndexedSlices(v, index, (7, 1))) for v in (view, plain))
+    assert torch.equal(got.values, want.values)
+    assert torch.equal(mpi.orthogonalize(view), mpi.orthogonalize(plain))
+    leaf = values(13, 7, 1).requires_grad_(True)
+    mpi.embedding(index, leaf).backward(view)
+    assert torch.equal(leaf.grad, mpi.embedding_gradient(plain, index, 7))
+    one, other = (torch.nn.Parameter(values(14, 30, 1)) for _ in range(2))
+    one.grad, other.grad = view, plain
+    mpi.Muon([one]).step(), mpi.Muon([other]).step()
+    assert torch.equal(one, other)
+    weight = torch.nn.Parameter(view)
+    weight.grad = torch.ones(30, 1).cuda()
+    with pytest.raises(mpi.InvalidArgumentError, match="negative"):
+        mpi.Muon([weight]).step()

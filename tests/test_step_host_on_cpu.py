@@ -183,3 +183,16 @@ def test_sides_of_nothing():
     lib = step_abi.lib()
     for m in (matrices((64, 256)), matrices((0, 500)), matrices()):
         assert [lib.step_orthogonalize_side(m, len(m), 0, k) for k in range(4)] == [0] * 4
+
+
+def test_views_that_stand_for_the_negative_of_their_memory(plain):
+    """The imaginary part of a conjugate is one: the kernels read memory, so it has to be made to hold the values."""
+    z = torch.randn(4, 1, dtype=torch.complex64)
+    weight = z.conj().imag
+    assert weight.is_neg()
+    assert torch.equal(mpi.embedding(IDS, weight), mpi.embedding(IDS, -z.imag))
+    leaf = z.conj().imag.resolve_neg().clone().requires_grad_(True)
+    grad = torch.randn(2, 3, 1, dtype=torch.complex64)
+    mpi.embedding(IDS, leaf).backward(grad.conj().imag)
+    assert torch.equal(leaf.grad, mpi.embedding_gradient(-grad.imag, IDS, 4))
+    assert torch.equal(mpi.embedding_gradient(grad.conj().imag, IDS, 4), leaf.grad)
