@@ -200,12 +200,11 @@ int main(int argc, char** argv) {
   if (!brief) {
     run({{{250, 64, 1}, {64, 256, 1}, {7, 9, 1}}, H, F, 1, 2, 0, false});
     run({{{1, 300, 1}, {300, 2, 1}, {64, 257, 1}}, F, F, 0, 3, 64, false});
-    run({{{257, 140, 1}}, H, H, 1, 2, 128, false});
+    run({{{200, 140, 1}}, H, H, 1, 2, 128, false});
     run({{{140, 321, 1}, {70, 100, 2}, {20, 30, 1}, {0, 900, 1}, {100, 100, 0}}, B, B, 0, 2, 128, true});
     run({{{140, 190, 1}, {20, 30, 2}, {64, 500, 1}}, F, F, 1, 1, 128, true});
     run({{{200, 210, 1}}, F, F, 0, 2, 192, false});
-    run({{{321, 200, 1}}, B, F, 0, 2, 256, false});
-    run({{{260, 330, 1}}, F, F, 0, 1, 256, true});
+    run({{{321, 200, 1}}, F, F, 0, 2, 256, true});
     // more batches, more shapes and more elements than a round holds
     run({{{5, 300, 1}, {6, 310, 1}, {7, 320, 1}, {320, 8, 1}}, F, F, 0, 1, 64, true});
     run({{{9, 300, 1}, {9, 400, 1}, {9, 450, 1}, {300, 9, 1}}, F, F, 1, 1, 64, false});
